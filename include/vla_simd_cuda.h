@@ -204,6 +204,114 @@ VLA_API int32_t vla_cuda_conv_transpose1d(float* out, const float* x, const floa
                                           int32_t T, int32_t Cin, int32_t Cout, int32_t k, int32_t stride,
                                           int32_t pad, void* stream);
 
+/* ------------------------------------------- prompts and the 4-bit cache
+ * The operators of a policy that is prompted with frames and text and answers
+ * token by token (or chunk by chunk): positions, attention over the prompt, a
+ * key / value cache, attention over the cache. No counterpart in the reference,
+ * whose policies run one fixed prefix per query. Device pointers unless said
+ * otherwise, asynchronous on `stream`.
+ *
+ * Heads are [tokens][heads][head_dim] with a token and a head stride in
+ * elements (so q, k and v may be views of one projection) and contiguous
+ * channels; outputs are contiguous. Element types are VLA_TYPE_*. A query head
+ * h reads key head h / (n_q / n_kv). Sums, maxima and norms are 32-bit. */
+#define VLA_TYPE_F32   0
+#define VLA_TYPE_F16   1
+#define VLA_TYPE_BF16  2
+
+/* Norm of each query and key head, and the rotary positions of several axes, in
+ * one pass. For a head x of head_dim channels: y = x * rsqrt(mean(x^2) + eps) *
+ * weight (q_weight / k_weight [head_dim] fp32; NULL: y = x). Then rot = 2 *
+ * sum(sections) channels turn: pair i is (y[i], y[i + rot/2]), the pairs of
+ * axis a are the next sections[a] ones, pos [n_axes][tokens] int32 holds the
+ * axis' positions, and the angle is pos * f_i with f_i = base^(-2i/rot), or
+ * base^(-j/sections[a]), j counted from the section's start, if restart != 0.
+ * Angles are formed in 64 bits. Channels past rot keep y. `sections` is a HOST
+ * array; 1 <= n_axes <= 4, rot <= head_dim <= 256, head_dim even. in_type and
+ * out_type may differ; outputs do not overlap inputs unless they are the very
+ * same elements (in place: same type, contiguous). n_kv = 0: queries alone (k
+ * and k_out may be NULL). tokens = 0 does nothing. */
+VLA_API int32_t vla_cuda_qk_norm_rope(void* q_out, void* k_out, int32_t out_type,
+                                      const void* q, int64_t q_tok, int64_t q_head,
+                                      const void* k, int64_t k_tok, int64_t k_head, int32_t in_type,
+                                      const int32_t* pos, const int32_t* sections, int32_t n_axes,
+                                      int32_t restart, const float* q_weight, const float* k_weight,
+                                      float eps, double base, int32_t tokens, int32_t n_q, int32_t n_kv,
+                                      int32_t head_dim, void* stream);
+
+/* Attention over n_seq prompts packed one after another: sequence s has the
+ * queries cu_q[s] .. cu_q[s+1] - 1 and the keys cu_k[s] .. cu_k[s+1] - 1 (int32
+ * [n_seq + 1], ascending; a sequence may be empty). Query i of lq sees the
+ * first n of its sequence's lk keys: n = lk, or with causal != 0 n = clamp(i + 1 +
+ * lk - lq, 0, lk) (the last query sees every key); with prefix (int32 [n_seq]
+ * or NULL) at least min(prefix[s], lk), so that a prompt's frames see one
+ * another. out [total_q][n_q][head_dim] = softmax(scale q.k) v; a query that
+ * sees nothing gives zeros, and keys and values it does not see do not reach it
+ * whatever they hold. Rows outside every sequence are not written. type F16 or
+ * BF16 (weights are rounded to it for the product with v); head_dim a multiple
+ * of 8, at most 128; addresses and strides of q, k, v multiples of 16 bytes. */
+VLA_API int32_t vla_cuda_prompt_attention(void* out, const void* q, int64_t q_tok, int64_t q_head,
+                                          const void* k, int64_t k_tok, int64_t k_head,
+                                          const void* v, int64_t v_tok, int64_t v_head, int32_t type,
+                                          const int32_t* cu_q, const int32_t* cu_k, const int32_t* prefix,
+                                          int32_t n_seq, int32_t total_q, int32_t total_k, int32_t n_q,
+                                          int32_t n_kv, int32_t head_dim, float scale, int32_t causal,
+                                          void* stream);
+
+/* The paged 4-bit key / value cache: cache [n_pages][n_kv][page / 16][20 *
+ * head_dim] bytes, 16-byte aligned; page 16, 32, 64, 128 or 256 tokens, head_dim
+ * 64 or 128. Slot = page index * page + position in the page.
+ *
+ * Per token, head and group of 32 channels: m = fp16(min), s = fp16((max - min)
+ * * (1/15)) (min and max clamped to +-65504), code = clamp(rne((x - m) / s), 0,
+ * 15) (0 where s = 0), value = code * s + m, each step one rounded 32-bit
+ * operation: 5 bits a value in all. A group that holds a NaN or an infinity
+ * gets s = m = NaN and reads as NaN.
+ *
+ * A block of 16 tokens (NG = head_dim / 32; keys: token t = 8 j + n; values and
+ * scales: t = 8 j + 2 quad + e), in order:
+ *   key codes    [j 2][n 8][quad 4][g NG]  uint32, nibble i: channel 32 g + 8 quad + i
+ *   key scales   [quad 4][g NG][j 2][e 2]  fp16
+ *   key minima   [n 8][j 2][g NG]          fp16
+ *   value codes  [j 2][n 8][quad 4][g NG]  uint32, nibble 4 e + i: channel 32 g + 4 n + i
+ *   value scales [quad 4][g NG][j 2][e 2]  fp16
+ *   value minima [quad 4][g NG][j 2][e 2]  fp16
+ *
+ * append writes k and v [tokens][n_kv] heads to slots [tokens] (int64; a
+ * negative slot is skipped; one past the cache is skipped and sets the device
+ * status word; two tokens of one call with the same slot leave either's bits).
+ * read gives the values of slots as k_out, v_out [tokens][n_kv][head_dim]
+ * (16-byte aligned), zeros for a skipped slot. */
+VLA_API int64_t vla_cuda_kv4_block_bytes(int32_t head_dim);
+VLA_API int32_t vla_cuda_kv4_append(void* cache, int64_t n_pages, int32_t page, const void* k, int64_t k_tok,
+                                    int64_t k_head, const void* v, int64_t v_tok, int64_t v_head, int32_t type,
+                                    const int64_t* slots, int32_t tokens, int32_t n_kv, int32_t head_dim,
+                                    void* stream);
+VLA_API int32_t vla_cuda_kv4_read(const void* cache, int64_t n_pages, int32_t page, void* k_out, void* v_out,
+                                  int32_t type, const int64_t* slots, int32_t tokens, int32_t n_kv,
+                                  int32_t head_dim, void* stream);
+
+/* Attention of new tokens over the 4-bit cache: q [batch][queries][n_q]
+ * heads (strides q_seq, q_tok, q_head), table [batch][table_ld] int32 page
+ * indices of which the first max_pages may be used, lens [batch] int32 tokens in
+ * the cache (clamped to max_pages * page). Query i of sequence b sees its first
+ * lens[b] tokens, or with causal != 0 the first clamp(lens[b] - queries + 1 + i,
+ * 0, lens[b]) (the new tokens are the last ones of the cache). out
+ * [batch][queries][n_q][head_dim], same type as q (any); a query that sees
+ * nothing gives zeros. A page index outside the cache is not read: its tokens
+ * are left out and the device status word is set. Bytes of the cache past
+ * lens[b] may hold anything. `ws`: workspace_bytes device bytes, 16-byte
+ * aligned (NULL where that is 0); calls that may overlap on the GPU need
+ * separate ones. */
+VLA_API uint64_t vla_cuda_kv4_attention_workspace_bytes(int32_t batch, int32_t queries, int32_t n_q, int32_t n_kv,
+                                                        int32_t head_dim, int32_t max_pages, int32_t page);
+VLA_API int32_t vla_cuda_kv4_attention(void* out, const void* q, int64_t q_seq, int64_t q_tok, int64_t q_head,
+                                       int32_t type, const void* cache, int64_t n_pages, int32_t page,
+                                       const int32_t* table, int64_t table_ld, int32_t max_pages,
+                                       const int32_t* lens, int32_t batch, int32_t queries, int32_t n_q,
+                                       int32_t n_kv, int32_t head_dim, float scale, int32_t causal, void* ws,
+                                       uint64_t ws_bytes, void* stream);
+
 /* ------------------------------------------------ host-pointer tcpu shims */
 
 VLA_API int32_t vla_tcpu_int8_gemm_available(void);          /* src/ops/quant_ops.h:41 */

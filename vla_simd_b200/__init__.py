@@ -95,6 +95,16 @@ SIGNATURES = {
     "vla_cuda_im2col1d": (I32, [VP, VP, I32, I32, I32, I32, I32, I32, VP]),
     "vla_cuda_conv_transpose1d": (I32, [VP, VP, VP, VP, I32, I32, I32, I32, I32, I32, VP]),
     "vla_cuda_dense_linear_f32": (I32, [VP, VP, VP, VP, I32, I32, I32, VP]),
+    "vla_cuda_qk_norm_rope": (I32, [VP, VP, I32, VP, I64, I64, VP, I64, I64, I32, VP, VP, I32, I32, VP, VP, F32,
+                                    ctypes.c_double, I32, I32, I32, I32, VP]),
+    "vla_cuda_prompt_attention": (I32, [VP, VP, I64, I64, VP, I64, I64, VP, I64, I64, I32, VP, VP, VP, I32, I32, I32,
+                                        I32, I32, I32, F32, I32, VP]),
+    "vla_cuda_kv4_block_bytes": (I64, [I32]),
+    "vla_cuda_kv4_append": (I32, [VP, I64, I32, VP, I64, I64, VP, I64, I64, I32, VP, I32, I32, I32, VP]),
+    "vla_cuda_kv4_read": (I32, [VP, I64, I32, VP, VP, I32, VP, I32, I32, I32, VP]),
+    "vla_cuda_kv4_attention_workspace_bytes": (ctypes.c_uint64, [I32, I32, I32, I32, I32, I32, I32]),
+    "vla_cuda_kv4_attention": (I32, [VP, VP, I64, I64, I64, I32, VP, I64, I32, VP, I64, I32, VP, I32, I32, I32, I32,
+                                     I32, F32, I32, VP, ctypes.c_uint64, VP]),
     "vla_tcpu_int8_gemm_available": (I32, []),
     "vla_tcpu_i8_kpad": (I32, [I32]),
     "vla_tcpu_packed_i8_words": (ctypes.c_uint64, [I32, I32]),

@@ -15,6 +15,7 @@
 #include "lm_ops.h"
 #include "nn.h"
 #include "quant.h"
+#include "serve_ops.h"
 
 #include <cuda_runtime.h>
 
@@ -743,6 +744,134 @@ int32_t vla_cuda_conv_transpose1d(float* out, const float* x, const float* W, co
         e = vsb::conv_transpose1d(x, W, bias, out, T, Cin, Cout, k, stride, pad, as_stream(stream));
     }
     return status_of(e);
+}
+
+// ------------------------------------------- prompts and the 4-bit cache
+
+static bool type_ok(int32_t type) { return type >= VLA_TYPE_F32 && type <= VLA_TYPE_BF16; }
+static bool heads_ok(int32_t n_q, int32_t n_kv) {
+    return n_q > 0 && n_kv > 0 && n_q % n_kv == 0 && n_q <= 65535;
+}
+static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+// a 16-bit operand that a tensor map can describe
+static bool tma_ok(const void* p, int64_t tok, int64_t head) {
+    return p && aligned16(p) && tok >= 0 && head >= 0 && tok % 8 == 0 && head % 8 == 0;
+}
+
+int32_t vla_cuda_qk_norm_rope(void* q_out, void* k_out, int32_t out_type, const void* q, int64_t q_tok, int64_t q_head,
+                              const void* k, int64_t k_tok, int64_t k_head, int32_t in_type, const int32_t* pos,
+                              const int32_t* sections, int32_t n_axes, int32_t restart, const float* q_weight,
+                              const float* k_weight, float eps, double base, int32_t tokens, int32_t n_q,
+                              int32_t n_kv, int32_t head_dim, void* stream) {
+    if (!type_ok(in_type) || !type_ok(out_type) || tokens < 0 || n_q < 0 || n_kv < 0 || n_q > 65535 || n_kv > 65535 ||
+        head_dim <= 0 || head_dim > 2 * vsb::kMaxPairs || head_dim % 2 || !sections || n_axes < 1 || n_axes > 4 ||
+        !(base > 0.0) || !std::isfinite(base) || !(eps >= 0.0f))
+        return VLA_ERR_ARG;
+    int64_t pairs = 0;
+    for (int32_t a = 0; a < n_axes; ++a) {
+        if (sections[a] < 1 || sections[a] > head_dim / 2) return VLA_ERR_ARG;
+        pairs += sections[a];
+    }
+    if (2 * pairs > head_dim) return VLA_ERR_ARG;
+    if (tokens == 0 || n_q + n_kv == 0) return VLA_OK;
+    if (!pos || (n_q > 0 && (!q || !q_out)) || (n_kv > 0 && (!k || !k_out))) return VLA_ERR_ARG;
+    vsb::RopeTable tab;
+    const double two_pi = 6.283185307179586476925286766559;
+    for (int32_t a = 0, i = 0; a < n_axes; ++a)
+        for (int32_t j = 0; j < sections[a]; ++j, ++i) {
+            const double at = restart ? (double)j / sections[a] : (double)i / (double)pairs;
+            tab.turns[i] = std::pow(base, -at) / two_pi;
+            tab.axis[i] = static_cast<unsigned char>(a);
+        }
+    return status_of(vsb::qk_norm_rope(q_out, k_out, out_type, {q, q_tok, q_head}, {k, k_tok, k_head}, in_type, pos,
+                                       tab, (int)(2 * pairs), q_weight, k_weight, eps, tokens, n_q, n_kv, head_dim,
+                                       as_stream(stream)));
+}
+
+int32_t vla_cuda_prompt_attention(void* out, const void* q, int64_t q_tok, int64_t q_head, const void* k, int64_t k_tok,
+                                  int64_t k_head, const void* v, int64_t v_tok, int64_t v_head, int32_t type,
+                                  const int32_t* cu_q, const int32_t* cu_k, const int32_t* prefix, int32_t n_seq,
+                                  int32_t total_q, int32_t total_k, int32_t n_q, int32_t n_kv, int32_t head_dim,
+                                  float scale, int32_t causal, void* stream) {
+    if ((type != VLA_TYPE_F16 && type != VLA_TYPE_BF16) || n_seq < 0 || total_q < 0 || total_k < 0 ||
+        !heads_ok(n_q, n_kv) || head_dim <= 0 || head_dim > 128 || head_dim % 8 || !std::isfinite(scale))
+        return VLA_ERR_ARG;
+    if (total_q == 0 || n_seq == 0) return VLA_OK;
+    if (!out || !aligned16(out) || !cu_q || !cu_k || !tma_ok(q, q_tok, q_head)) return VLA_ERR_ARG;
+    if (total_k > 0 && (!tma_ok(k, k_tok, k_head) || !tma_ok(v, v_tok, v_head))) return VLA_ERR_ARG;
+    return status_of(vsb::prompt_attention(out, {q, q_tok, q_head}, {k, k_tok, k_head}, {v, v_tok, v_head}, type, cu_q,
+                                           cu_k, prefix, n_seq, total_q, total_k, n_q, n_kv, head_dim, scale,
+                                           causal != 0, as_stream(stream)));
+}
+
+static bool kv4_ok(const void* cache, int64_t n_pages, int32_t page, int32_t n_kv, int32_t head_dim) {
+    return cache && aligned16(cache) && n_pages > 0 && page >= 16 && page <= 256 && (page & (page - 1)) == 0 &&
+           n_kv > 0 && n_kv <= 65535 && (head_dim == 64 || head_dim == 128) && n_pages <= INT32_MAX / page;
+}
+
+int64_t vla_cuda_kv4_block_bytes(int32_t head_dim) { return head_dim == 64 || head_dim == 128 ? 20 * head_dim : 0; }
+
+int32_t vla_cuda_kv4_append(void* cache, int64_t n_pages, int32_t page, const void* k, int64_t k_tok, int64_t k_head,
+                            const void* v, int64_t v_tok, int64_t v_head, int32_t type, const int64_t* slots,
+                            int32_t tokens, int32_t n_kv, int32_t head_dim, void* stream) {
+    if (!kv4_ok(cache, n_pages, page, n_kv, head_dim) || !type_ok(type) || tokens < 0) return VLA_ERR_ARG;
+    if (tokens == 0) return VLA_OK;
+    if (!k || !v || !slots) return VLA_ERR_ARG;
+    const vsb::Kv4Cache c{static_cast<uint8_t*>(cache), n_pages, page, n_kv, head_dim};
+    return status_of(vsb::kv4_append(c, {k, k_tok, k_head}, {v, v_tok, v_head}, type,
+                                     reinterpret_cast<const long long*>(slots), tokens, as_stream(stream)));
+}
+
+int32_t vla_cuda_kv4_read(const void* cache, int64_t n_pages, int32_t page, void* k_out, void* v_out, int32_t type,
+                          const int64_t* slots, int32_t tokens, int32_t n_kv, int32_t head_dim, void* stream) {
+    if (!kv4_ok(cache, n_pages, page, n_kv, head_dim) || !type_ok(type) || tokens < 0) return VLA_ERR_ARG;
+    if (tokens == 0) return VLA_OK;
+    if (!k_out || !v_out || !aligned16(k_out) || !aligned16(v_out) || !slots) return VLA_ERR_ARG;
+    const vsb::Kv4Cache c{static_cast<uint8_t*>(const_cast<void*>(cache)), n_pages, page, n_kv, head_dim};
+    return status_of(vsb::kv4_read(c, k_out, v_out, type, reinterpret_cast<const long long*>(slots), tokens,
+                                   as_stream(stream)));
+}
+
+uint64_t vla_cuda_kv4_attention_workspace_bytes(int32_t batch, int32_t queries, int32_t n_q, int32_t n_kv,
+                                                int32_t head_dim, int32_t max_pages, int32_t page) {
+    if (!heads_ok(n_q, n_kv) || max_pages <= 0 || page <= 0) return 0;
+    return vsb::kv4_attention_ws_bytes(batch, queries, n_q, n_kv, head_dim, (long long)max_pages * page);
+}
+
+int32_t vla_cuda_kv4_attention(void* out, const void* q, int64_t q_seq, int64_t q_tok, int64_t q_head, int32_t type,
+                               const void* cache, int64_t n_pages, int32_t page, const int32_t* table,
+                               int64_t table_ld, int32_t max_pages, const int32_t* lens, int32_t batch,
+                               int32_t queries, int32_t n_q, int32_t n_kv, int32_t head_dim, float scale,
+                               int32_t causal, void* ws, uint64_t ws_bytes, void* stream) {
+    if (!kv4_ok(cache, n_pages, page, n_kv, head_dim) || !type_ok(type) || !heads_ok(n_q, n_kv) || batch < 0 ||
+        batch > 65535 || queries < 0 || max_pages < 0 || max_pages > INT32_MAX / page || table_ld < max_pages ||
+        !std::isfinite(scale))
+        return VLA_ERR_ARG;
+    if (batch == 0 || queries == 0) return VLA_OK;
+    if ((int64_t)queries * (n_q / n_kv) > INT32_MAX / 16 ||
+        ((int64_t)queries * (n_q / n_kv) + 7) / 8 * n_kv > 65535)
+        return VLA_ERR_SHAPE;
+    if (!out || !q || !lens || (max_pages > 0 && !table) || !aligned16(ws)) return VLA_ERR_ARG;
+    vsb::Kv4AttArgs a;
+    a.out = out;
+    a.q = q;
+    a.q_seq = q_seq;
+    a.q_tok = q_tok;
+    a.q_head = q_head;
+    a.type = type;
+    a.cache = {static_cast<uint8_t*>(const_cast<void*>(cache)), n_pages, page, n_kv, head_dim};
+    a.table = table;
+    a.table_ld = table_ld;
+    a.max_pages = max_pages;
+    a.lens = lens;
+    a.batch = batch;
+    a.queries = queries;
+    a.n_q = n_q;
+    a.scale = scale;
+    a.causal = causal != 0;
+    a.ws = ws;
+    a.ws_bytes = ws_bytes;
+    return status_of(vsb::kv4_attention(a, as_stream(stream)));
 }
 
 // ------------------------------------------------------ host-pointer shims

@@ -10,3 +10,6 @@
 #include "dp.cu"
 #include "octo.cu"
 #include "smolvla.cu"
+#include "serve_ops.cu"
+#include "attn_kv4.cu"
+#include "attn_prompt.cu"
