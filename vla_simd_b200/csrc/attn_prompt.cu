@@ -1,8 +1,31 @@
 // Attention over packed prompts: grouped heads, causal or dense, sequences of
 // different lengths one after another in one array.
+//
+// One pass over the keys with the running maximum m and sum l of a softmax:
+//   S = Q K^T;  P = 2^(c (S - m)), c = scale log2(e);  l += rowsum P;  O += P V
+// both products on tcgen05 (128 x 128 x D, accumulators in TMEM), P written back
+// over S's columns as the A operand of the second one, so scores and weights
+// never leave the SM.
+//
+// A CTA has two 128-row tiles of one key head. A tile's rows are (query, head of
+// the group) pairs, token-major: the keys of a group are loaded once for all of
+// its heads, and a causal tile spans 128 / group tokens, which keeps what the
+// mask throws away small. Warps: 0-3 and 4-7 the softmax of tile 0 and 1 (thread
+// = row = TMEM lane), 8 issues the matrix products, 9 the TMA loads of a ring of
+// K and V tiles. While one tile's softmax runs, the tensor core has the other's
+// products.
+//
+// m only follows the true maximum when it is more than 2^8 behind (P then stays
+// below 2^8, far inside bf16 and fp16): O is rescaled in TMEM that rarely, by
+// the softmax threads themselves.
 #include "serve_ops.h"
+#include "gemm_i8.h"
 #include "launch.cuh"
 #include "sm100.cuh"
+
+#include <atomic>
+#include <climits>
+#include <type_traits>
 
 namespace vsb {
 
@@ -12,8 +35,9 @@ struct PromptArgs {
     HeadsIn q, k, v;
     void* out;
     const int *cu_q, *cu_k, *prefix;
-    int n_seq, total_q, total_k, n_q, n_kv, d, causal;
-    float scale_log2;   // scale * log2(e)
+    int n_seq, total_q, total_k, n_q, n_kv, d, causal, negate;
+    float scale_log2;   // |scale| * log2(e)
+    int gp, tile_tok;   // heads and tokens of a 128-row tile
 };
 
 // keys that query i of a sequence of lq queries and lk keys sees: [0, limit)
@@ -23,42 +47,33 @@ __device__ __forceinline__ int prompt_limit(const PromptArgs& a, int seq, int i,
     return lim;
 }
 
-// One warp a row, one key at a time: the definition with an online softmax.
+// One row by one warp, one key at a time: the definition. It serves the rows
+// whose tile holds a NaN or an infinity in a value that the mask hides from some
+// of its rows (0 * NaN would reach them through the matrix product).
 template <typename T>
-__global__ void __launch_bounds__(128)
-prompt_row_kernel(const __grid_constant__ PromptArgs a) {
-    const int lane = threadIdx.x & 31, row = blockIdx.x * 4 + (threadIdx.x >> 5), head = blockIdx.y;
-    pdl_trigger();
-    pdl_wait();
-    if (row >= a.total_q) return;
-    int seq = 0;
-    while (seq < a.n_seq && a.cu_q[seq + 1] <= row) ++seq;
-    if (seq >= a.n_seq || row < a.cu_q[seq]) return;
+__device__ __noinline__ void prompt_row(const PromptArgs& a, int row, int head, int k0, int lim) {
+    const int lane = threadIdx.x & 31, kvh = head / (a.n_q / a.n_kv);
     float o[4] = {}, q[4] = {}, m = -INFINITY, l = 0.f;
-    {
-        const int q0 = a.cu_q[seq], k0 = max(a.cu_k[seq], 0), k1 = min(a.cu_k[seq + 1], a.total_k);
-        const int kvh = head / (a.n_q / a.n_kv);
-        const int lim = prompt_limit(a, seq, row - q0, a.cu_q[seq + 1] - q0, max(k1 - k0, 0));
-        const T* qp = static_cast<const T*>(a.q.p) + (long long)row * a.q.tok + (long long)head * a.q.head;
+    const T* qp = static_cast<const T*>(a.q.p) + (long long)row * a.q.tok + (long long)head * a.q.head;
+    const float c = a.negate ? -a.scale_log2 : a.scale_log2;
+    #pragma unroll
+    for (int x = 0; x < 4; ++x)
+        if (lane + 32 * x < a.d) q[x] = to_f(qp[lane + 32 * x]);
+    for (int j = 0; j < lim; ++j) {
+        const T* kp = static_cast<const T*>(a.k.p) + (long long)(k0 + j) * a.k.tok + (long long)kvh * a.k.head;
+        const T* vp = static_cast<const T*>(a.v.p) + (long long)(k0 + j) * a.v.tok + (long long)kvh * a.v.head;
+        float s = 0.f;
         #pragma unroll
         for (int x = 0; x < 4; ++x)
-            if (lane + 32 * x < a.d) q[x] = to_f(qp[lane + 32 * x]);
-        for (int j = 0; j < lim; ++j) {
-            const T* kp = static_cast<const T*>(a.k.p) + (long long)(k0 + j) * a.k.tok + (long long)kvh * a.k.head;
-            const T* vp = static_cast<const T*>(a.v.p) + (long long)(k0 + j) * a.v.tok + (long long)kvh * a.v.head;
-            float s = 0.f;
-            #pragma unroll
-            for (int x = 0; x < 4; ++x)
-                if (lane + 32 * x < a.d) s = fmaf(q[x], to_f(kp[lane + 32 * x]), s);
-            for (int y = 16; y > 0; y >>= 1) s += __shfl_xor_sync(0xffffffffu, s, y);
-            s *= a.scale_log2;
-            const float mn = fmaxf(m, s), alpha = ex2(m - mn), w = ex2(s - mn);
-            m = mn;
-            l = fmaf(l, alpha, w);
-            #pragma unroll
-            for (int x = 0; x < 4; ++x)
-                if (lane + 32 * x < a.d) o[x] = fmaf(o[x], alpha, w * to_f(vp[lane + 32 * x]));
-        }
+            if (lane + 32 * x < a.d) s = fmaf(q[x], to_f(kp[lane + 32 * x]), s);
+        for (int y = 16; y > 0; y >>= 1) s += __shfl_xor_sync(0xffffffffu, s, y);
+        s *= c;
+        const float mn = fmaxf(m, s), alpha = ex2(m - mn), w = ex2(s - mn);
+        m = mn;
+        l = fmaf(l, alpha, w);
+        #pragma unroll
+        for (int x = 0; x < 4; ++x)
+            if (lane + 32 * x < a.d) o[x] = fmaf(o[x], alpha, w * to_f(vp[lane + 32 * x]));
     }
     const float inv = l == 0.f ? 0.f : 1.0f / l;
     T* out = static_cast<T*>(a.out) + ((long long)row * a.n_q + head) * a.d;
@@ -67,18 +82,500 @@ prompt_row_kernel(const __grid_constant__ PromptArgs a) {
         if (lane + 32 * x < a.d) out[lane + 32 * x] = from_f<T>(o[x] * inv);
 }
 
+constexpr int kPaThreads = 384, kPaRows = 128, kPaKeys = 128;
+// registers a thread: the softmax warpgroups take what the third one gives up
+constexpr int kPaRegsSoftmax = 208, kPaRegsRest = 88, kPaRegsAtLaunch = (2 * kPaRegsSoftmax + kPaRegsRest) / 3;
+constexpr uint32_t kPaBoxBytes = 128 * 128;   // 128 rows of 64 channels
+
+__host__ __device__ constexpr int pa_stages(int D) { return D == 128 ? 5 : 8; }
+constexpr size_t pa_smem(int D) { return 1024 + (size_t)(2 + pa_stages(D)) * (D / 64) * kPaBoxBytes + 512; }
+
+// kind::f16 instruction descriptor: F32 accumulator, A and B both bf16 or both
+// fp16, M = 128; b_mn: B is stored with its N index innermost
+__host__ __device__ constexpr uint32_t idesc_f16(bool bf16, int N, bool b_mn, bool neg_a) {
+    return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((neg_a ? 1u : 0u) << 13) |
+           ((b_mn ? 1u : 0u) << 16) | (static_cast<uint32_t>(N >> 3) << 17) | (8u << 24);
+}
+
+__device__ __forceinline__ void umma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                 :: "r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+}
+__device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+                 :: "r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+}
+
+// Descriptor of a V tile as the B operand with N (channels) innermost: rows of
+// 64 channels (128 bytes, swizzled), 8-key groups 1024 bytes apart (SBO), blocks
+// of 64 channels 16384 bytes apart (LBO).
+__device__ __forceinline__ uint64_t sw128_mnmajor_desc(uint32_t saddr) {
+    return static_cast<uint64_t>((saddr & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(kPaBoxBytes >> 4) << 16) |
+           (static_cast<uint64_t>(1024u >> 4) << 32) | (static_cast<uint64_t>(1u) << 46) |
+           (static_cast<uint64_t>(2u) << 61);
+}
+
+__device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};"
+        :: "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+           "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]),
+           "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
+           "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};"
+        :: "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+           "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+template <int N>
+__device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(N)); }
+template <int N>
+__device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(N)); }
+
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;"
+        : "=l"(reinterpret_cast<unsigned long long&>(d))
+        : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)),
+          "l"(reinterpret_cast<unsigned long long&>(c)));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("add.rn.f32x2 %0, %1, %2;"
+        : "=l"(reinterpret_cast<unsigned long long&>(d))
+        : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
+    return d;
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) { return pack_h2(lo, hi); }
+
+// What a CTA works on: tile t has rows of queries [tok[t], tok[t] + n_tok[t])
+// of the sequence and sees the first keys[t] of its lk keys.
+struct PromptJob {
+    int seq, q0, lq, k0, lk, tok[2], n_tok[2], keys[2], bad;
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kPaThreads, 1)
+prompt_tc_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__ CUtensorMap mq,
+                 const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv) {
+    constexpr bool kBf16 = sizeof(T) == 2 && !std::is_same<T, __half>::value;
+    constexpr int kStages = pa_stages(D), kCB = D / 64;
+    constexpr uint32_t kTile = kCB * kPaBoxBytes;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* sm = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    uint8_t* sq = sm;                       // two Q tiles
+    uint8_t* ring = sm + 2 * kTile;
+    uint64_t* q_full = reinterpret_cast<uint64_t*>(ring + kStages * kTile);
+    uint64_t* kv_full = q_full + 1;
+    uint64_t* kv_empty = kv_full + kStages;
+    uint64_t* s_full = kv_empty + kStages;
+    uint64_t* p_full = s_full + 2;
+    uint64_t* o_done = p_full + 2;
+    uint32_t* tslot = reinterpret_cast<uint32_t*>(o_done + 2);
+    PromptJob* job = reinterpret_cast<PromptJob*>(tslot + 2);
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int head_blocks = a.n_q / a.gp;
+    const int hb = blockIdx.x % head_blocks;
+    const int head0 = hb * a.gp, kvh = head0 / (a.n_q / a.n_kv);
+    if (tid == 0) {
+        mbar_init(q_full, 1);
+        for (int i = 0; i < kStages; ++i) {
+            mbar_init(kv_full + i, 1);
+            mbar_init(kv_empty + i, 1);
+        }
+        for (int t = 0; t < 2; ++t) {
+            mbar_init(s_full + t, 1);
+            mbar_init(p_full + t, 128);
+            mbar_init(o_done + t, 1);
+        }
+        fence_mbar_init();
+        tma_prefetch_desc(&mq);
+        tma_prefetch_desc(&mk);
+        tma_prefetch_desc(&mv);
+    }
+    if (warp == 8) tmem_alloc(tslot, 512);
+    pdl_wait();
+    if (warp == 0) {
+        // the sequence this CTA's pair of tiles lies in: pairs are numbered by
+        // sequence, and within one from its end, the rows with the most keys first
+        int want = blockIdx.x / head_blocks, found = -1, at = 0;
+        for (int s0 = 0; s0 < a.n_seq && found < 0; s0 += 32) {
+            const int s = s0 + lane;
+            int n = 0;
+            if (s < a.n_seq) {
+                const int lo = min(max(a.cu_q[s], 0), a.total_q), hi = min(max(a.cu_q[s + 1], lo), a.total_q);
+                n = (hi - lo + 2 * a.tile_tok - 1) / (2 * a.tile_tok);
+            }
+            int sum = n;
+            for (int o = 1; o < 32; o <<= 1) {
+                const int x = __shfl_up_sync(0xffffffffu, sum, o);
+                if (lane >= o) sum += x;
+            }
+            const unsigned hit = __ballot_sync(0xffffffffu, want < sum);
+            if (hit) {
+                const int l = __ffs(hit) - 1;
+                found = s0 + l;
+                at = __shfl_sync(0xffffffffu, sum, l) - 1 - want;   // pairs after this one
+            } else {
+                want -= __shfl_sync(0xffffffffu, sum, 31);
+            }
+        }
+        if (lane == 0) {
+            PromptJob j = {};
+            j.seq = found;
+            if (found >= 0) {
+                j.q0 = min(max(a.cu_q[found], 0), a.total_q);
+                j.lq = min(max(a.cu_q[found + 1], j.q0), a.total_q) - j.q0;
+                j.k0 = min(max(a.cu_k[found], 0), a.total_k);
+                j.lk = min(max(a.cu_k[found + 1], j.k0), a.total_k) - j.k0;
+                for (int t = 0; t < 2; ++t) {
+                    j.tok[t] = (2 * at + t) * a.tile_tok;
+                    j.n_tok[t] = min(max(j.lq - j.tok[t], 0), a.tile_tok);
+                    j.keys[t] = j.n_tok[t] > 0 ? prompt_limit(a, found, j.tok[t] + j.n_tok[t] - 1, j.lq, j.lk) : 0;
+                }
+            }
+            *job = j;
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    pdl_trigger();
+    const uint32_t tmem = *tslot;
+    const int seq = job->seq;
+    const int nblk0 = (job->keys[0] + kPaKeys - 1) / kPaKeys, nblk1 = (job->keys[1] + kPaKeys - 1) / kPaKeys;
+    const int nblk = max(nblk0, nblk1);
+
+    if (warp >= 8) {
+        regs_dec<kPaRegsRest>();
+        if (warp == 9 && nblk > 0) {
+            // ---- loads: Q tiles, then K and V of each block through the ring
+            if (lane == 0) {
+                mbar_arrive_expect_tx(q_full, (uint32_t)((nblk0 > 0) + (nblk1 > 0)) * kCB * 128u * (uint32_t)(a.gp * a.tile_tok));
+                for (int t = 0; t < 2; ++t)
+                    if ((t ? nblk1 : nblk0) > 0)
+                        for (int c = 0; c < kCB; ++c)
+                            tma_load_3d(sq + t * kTile + c * kPaBoxBytes, &mq, q_full, 64 * c, head0, job->q0 + job->tok[t]);
+                int i = 0;
+                for (; i < 2 * nblk; ++i) {
+                    const int st = i % kStages;
+                    if (i >= kStages && !mbar_wait(kv_empty + st, (uint32_t)(i / kStages - 1) & 1u)) break;
+                    mbar_arrive_expect_tx(kv_full + st, kTile);
+                    for (int c = 0; c < kCB; ++c)
+                        tma_load_3d(ring + st * kTile + c * kPaBoxBytes, (i & 1) ? &mv : &mk, kv_full + st, 64 * c, kvh,
+                                    job->k0 + (i >> 1) * kPaKeys);
+                }
+                // every copy has landed before the CTA may leave (after a wait that gave up, too)
+                const uint64_t until = globaltimer_ns() + kWaitLimitNs;
+                mbar_wait_until(q_full, 0, until);
+                for (int x = max(0, i - kStages); x < i; ++x)
+                    mbar_wait_until(kv_full + x % kStages, (uint32_t)(x / kStages) & 1u, until);
+            }
+        } else if (warp == 8 && nblk > 0) {
+            // ---- matrix products
+            constexpr uint32_t kPV = idesc_f16(kBf16, D, true, false);
+            const uint32_t kQK = a.negate ? idesc_f16(kBf16, kPaKeys, false, true) : idesc_f16(kBf16, kPaKeys, false, false);
+            // the fewest keys any row here sees: past them some weights are masked to 0
+            const int first_tok = job->n_tok[0] > 0 ? job->tok[0] : job->tok[1];
+            const int clear = prompt_limit(a, seq, first_tok, job->lq, job->lk);
+            auto wait = [](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)) != 0; };
+            bool ok = wait(q_full, 0);
+            auto qk = [&](int t, int j) {
+                const int i = 2 * j, st = i % kStages;
+                ok = ok && wait(kv_full + st, (uint32_t)(i / kStages) & 1u);
+                if (!ok) return;
+                tc_fence_after();
+                if (lane == 0) {
+                    const uint32_t qa = smem_u32(sq + t * kTile), kb = smem_u32(ring + st * kTile);
+                    #pragma unroll
+                    for (int k = 0; k < D / 16; ++k)
+                        umma_f16_ss(tmem + 128 * t, sw128_kmajor_desc(qa + (k >> 2) * kPaBoxBytes + (k & 3) * 32),
+                                    sw128_kmajor_desc(kb + (k >> 2) * kPaBoxBytes + (k & 3) * 32), kQK, k > 0);
+                    umma_commit(s_full + t);
+                }
+                __syncwarp();
+            };
+            if (nblk0 > 0) qk(0, 0);
+            if (nblk1 > 0) qk(1, 0);
+            if (lane == 0 && ok) umma_commit(kv_empty + 0);
+            int scrubbed = -1;
+            for (int j = 0; j < nblk && ok; ++j) {
+                const int iv = 2 * j + 1, sv = iv % kStages;
+                for (int t = 0; t < 2 && ok; ++t) {
+                    const int nb = t ? nblk1 : nblk0;
+                    if (j < nb) {
+                        ok = wait(kv_full + sv, (uint32_t)(iv / kStages) & 1u);
+                        if (ok && scrubbed < j && (j + 1) * kPaKeys > clear) {
+                            // a block that some row does not see all of: 0 * v has to be 0. Rows past the
+                            // sequence become zeros; a NaN or an infinity in front of its end is left to
+                            // the rows that see it, and the others are done again one by one.
+                            scrubbed = j;
+                            uint8_t* vt = ring + sv * kTile;
+                            const int valid = min(job->lk - j * kPaKeys, kPaKeys);
+                            constexpr uint32_t kExp = kBf16 ? 0x7F80u : 0x7C00u;
+                            bool bad = false;
+                            for (int c = 0; c < kCB; ++c)
+                                for (int x = lane; x < (int)kPaBoxBytes / 16; x += 32) {
+                                    uint4* p = reinterpret_cast<uint4*>(vt + c * kPaBoxBytes) + x;
+                                    if (x >= valid * 8) {
+                                        *p = make_uint4(0u, 0u, 0u, 0u);
+                                    } else {
+                                        const uint4 w = *p;
+                                        const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+                                        #pragma unroll
+                                        for (int y = 0; y < 4; ++y)
+                                            bad |= (ws[y] & kExp) == kExp || (ws[y] >> 16 & kExp) == kExp;
+                                    }
+                                }
+                            if (bad) job->bad = 1;
+                            __threadfence_block();
+                            fence_proxy_async_smem();
+                            __syncwarp();
+                        }
+                        ok = ok && wait(p_full + t, (uint32_t)j & 1u);
+                        if (!ok) break;
+                        tc_fence_after();
+                        if (lane == 0) {
+                            const uint32_t va = smem_u32(ring + sv * kTile);
+                            #pragma unroll
+                            for (int k = 0; k < kPaKeys / 16; ++k)
+                                umma_f16_ts(tmem + 256 + 128 * t, tmem + 128 * t + 8 * k, sw128_mnmajor_desc(va + k * 2048),
+                                            kPV, j > 0 || k > 0);
+                            umma_commit(o_done + t);
+                        }
+                        __syncwarp();
+                    }
+                    if (j + 1 < nb) qk(t, j + 1);
+                }
+                if (lane == 0 && ok) {
+                    umma_commit(kv_empty + sv);
+                    if (j + 1 < nblk) umma_commit(kv_empty + (2 * j + 2) % kStages);
+                }
+                __syncwarp();
+            }
+        }
+    } else {
+        regs_inc<kPaRegsSoftmax>();
+        // ---- softmax: thread = row
+        const int t = warp >> 2, r = tid & 127;
+        const int nb = t ? nblk1 : nblk0;
+        const int rt = r / a.gp, rg = r - rt * a.gp;
+        const bool live = rt < job->n_tok[t] && seq >= 0;
+        const int lim = live ? prompt_limit(a, seq, job->tok[t] + rt, job->lq, job->lk) : 0;
+        const int clear = nb > 0 ? prompt_limit(a, seq, job->tok[t], job->lq, job->lk) : 0;   // fewest keys of the tile
+        const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
+        const uint32_t tS = tmem + 128 * t + lane_base, tO = tmem + 256 + 128 * t + lane_base;
+        const float c = a.scale_log2, slack = 8.0f / c;
+        float m = -INFINITY, l = 0.f;
+        bool ok = true;
+        for (int j = 0; j < nb; ++j) {
+            ok = mbar_wait(s_full + t, (uint32_t)j & 1u);
+            if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+            tc_fence_after();
+            uint32_t s[4][32];
+            #pragma unroll
+            for (int x = 0; x < 4; ++x) tmem_ld_32x32b_x32(tS + 32 * x, s[x]);
+            tmem_ld_wait();
+            if ((j + 1) * kPaKeys > clear) {
+                const int left = lim - j * kPaKeys;
+                #pragma unroll
+                for (int x = 0; x < 128; ++x)
+                    if (x >= left) s[x >> 5][x & 31] = 0xFF800000u;   // -inf
+            }
+            float mx[4];
+            #pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                mx[x] = __uint_as_float(s[x][0]);
+                #pragma unroll
+                for (int y = 1; y < 32; ++y) mx[x] = fmaxf(mx[x], __uint_as_float(s[x][y]));
+            }
+            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+            if (__any_sync(0xffffffffu, top > m + slack || (m == -INFINITY && top > m))) {
+                const float mn = fmaxf(m, top);
+                if (j > 0) {
+                    // rescale O once the products so far are in
+                    ok = mbar_wait(o_done + t, (uint32_t)(j - 1) & 1u);
+                    if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+                    tc_fence_after();
+                    const float alpha = m == -INFINITY ? 0.f : ex2((m - mn) * c);
+                    l *= alpha;
+                    #pragma unroll 1
+                    for (int x = 0; x < D / 16; ++x) {
+                        uint32_t o[16];
+                        tmem_ld_32x32b_x16(tO + 16 * x, o);
+                        tmem_ld_wait();
+                        #pragma unroll
+                        for (int y = 0; y < 16; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * alpha);
+                        tmem_st_32x32b_x16(tO + 16 * x, o);
+                    }
+                    tmem_st_wait();
+                }
+                m = mn;
+            }
+            const float mc = m == -INFINITY ? 0.f : -m * c;
+            const float2 c2 = make_float2(c, c), mc2 = make_float2(mc, mc);
+            float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+            #pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                uint32_t p[32];
+                #pragma unroll
+                for (int x = 0; x < 32; ++x) {
+                    const int e = 64 * half + 2 * x;
+                    float2 v = fma2(make_float2(__uint_as_float(s[e >> 5][e & 31]), __uint_as_float(s[e >> 5][(e & 31) + 1])),
+                                    c2, mc2);
+                    v.x = ex2(v.x);
+                    v.y = ex2(v.y);
+                    sum[x & 1] = add2(sum[x & 1], v);
+                    p[x] = pack2<T>(v.x, v.y);
+                }
+                tmem_st_32x32b_x32(tS + 32 * half, p);
+            }
+            l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+            tmem_st_wait();
+            tc_fence_before();
+            mbar_arrive(p_full + t);
+        }
+        // ---- O / l
+        if (ok && nb > 0) ok = mbar_wait(o_done + t, (uint32_t)(nb - 1) & 1u);
+        ok = __all_sync(0xffffffffu, ok);
+        if (ok) {
+            tc_fence_after();
+            const float inv = nb > 0 && l != 0.f ? 1.0f / l : 0.f;
+            T* out = static_cast<T*>(a.out) + ((long long)(job->q0 + job->tok[t] + rt) * a.n_q + head0 + rg) * a.d;
+            #pragma unroll 1
+            for (int x = 0; x < D / 32; ++x) {
+                uint32_t o[32];
+                if (nb > 0) {
+                    tmem_ld_32x32b_x32(tO + 32 * x, o);
+                    tmem_ld_wait();
+                }
+                if (!live) continue;
+                #pragma unroll
+                for (int y = 0; y < 4; ++y) {
+                    if (32 * x + 8 * y >= a.d) break;
+                    uint4 w = make_uint4(0u, 0u, 0u, 0u);
+                    if (nb > 0 && lim > 0) {
+                        w.x = pack2<T>(__uint_as_float(o[8 * y]) * inv, __uint_as_float(o[8 * y + 1]) * inv);
+                        w.y = pack2<T>(__uint_as_float(o[8 * y + 2]) * inv, __uint_as_float(o[8 * y + 3]) * inv);
+                        w.z = pack2<T>(__uint_as_float(o[8 * y + 4]) * inv, __uint_as_float(o[8 * y + 5]) * inv);
+                        w.w = pack2<T>(__uint_as_float(o[8 * y + 6]) * inv, __uint_as_float(o[8 * y + 7]) * inv);
+                    }
+                    *reinterpret_cast<uint4*>(out + 32 * x + 8 * y) = w;
+                }
+            }
+            if (nb > 0 && *reinterpret_cast<volatile int*>(&job->bad)) {
+                __syncwarp();
+                for (int x = 0; x < 32; ++x) {
+                    const int xr = __shfl_sync(0xffffffffu, rt, x), xg = __shfl_sync(0xffffffffu, rg, x);
+                    const int xl = __shfl_sync(0xffffffffu, lim, x);
+                    if (__shfl_sync(0xffffffffu, (int)live, x))
+                        prompt_row<T>(a, job->q0 + job->tok[t] + xr, head0 + xg, job->k0, xl);
+                }
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 8) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+// Tensor map of [tokens][heads][d] 16-bit elements: boxes of 64 channels (zeros
+// past d) x box_heads x box_tok, rows of 128 bytes swizzled.
+bool make_tmap_heads(CUtensorMap* map, const HeadsIn& h, int tokens, int heads, int d, int box_heads, int box_tok,
+                     bool bf16) {
+    auto fn = get_encode_fn();
+    if (!fn || tokens <= 0) return false;
+    // a stride that is never taken still has to be a legal one
+    const long long head = heads > 1 ? h.head : d, tok = tokens > 1 ? h.tok : (long long)heads * head;
+    if ((reinterpret_cast<uintptr_t>(h.p) & 15) || head <= 0 || tok <= 0 || head % 8 || tok % 8) return false;
+    const cuuint64_t dims[3] = {(cuuint64_t)d, (cuuint64_t)heads, (cuuint64_t)tokens};
+    const cuuint64_t strides[2] = {(cuuint64_t)head * 2, (cuuint64_t)tok * 2};
+    const cuuint32_t box[3] = {64, (cuuint32_t)box_heads, (cuuint32_t)box_tok};
+    const cuuint32_t estr[3] = {1, 1, 1};
+    return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(h.p),
+              dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int D>
+cudaError_t prompt_launch(const PromptArgs& a, cudaStream_t st) {
+    static std::atomic<unsigned long long> ready{0};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const unsigned long long bit = 1ull << (dev & 63);
+    if (!(ready.load() & bit)) {
+        e = cudaFuncSetAttribute(prompt_tc_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pa_smem(D));
+        if (e != cudaSuccess) return e;
+        // the split of the registers must not ask for more than the block is launched with
+        cudaFuncAttributes fa;
+        e = cudaFuncGetAttributes(&fa, prompt_tc_kernel<T, D>);
+        if (e != cudaSuccess) return e;
+        if (fa.numRegs < kPaRegsAtLaunch) return cudaErrorInvalidConfiguration;
+        ready.fetch_or(bit);
+    }
+    CUtensorMap mq, mk, mv;
+    constexpr bool bf16 = !std::is_same<T, __half>::value;
+    if (!make_tmap_heads(&mq, a.q, a.total_q, a.n_q, a.d, a.gp, a.tile_tok, bf16)) return cudaErrorInvalidValue;
+    if (a.total_k > 0) {
+        if (!make_tmap_heads(&mk, a.k, a.total_k, a.n_kv, a.d, 1, kPaKeys, bf16) ||
+            !make_tmap_heads(&mv, a.v, a.total_k, a.n_kv, a.d, 1, kPaKeys, bf16))
+            return cudaErrorInvalidValue;
+    } else {
+        mk = mv = mq;   // no key is loaded
+    }
+    // a sequence's last pair may be short: at most one more pair each than the tokens fill
+    const long long pairs = (a.total_q + 2ll * a.tile_tok - 1) / (2 * a.tile_tok) + a.n_seq;
+    const long long grid = pairs * (a.n_q / a.gp);
+    if (grid > INT_MAX) return cudaErrorInvalidValue;
+    return launch_k(prompt_tc_kernel<T, D>, dim3((unsigned)grid), dim3(kPaThreads), pa_smem(D), st, a, mq, mk, mv);
+}
+
 }  // namespace
 
 cudaError_t prompt_attention(void* out, const HeadsIn& q, const HeadsIn& k, const HeadsIn& v, int type,
                              const int* cu_q, const int* cu_k, const int* prefix, int n_seq, int total_q, int total_k,
                              int n_q, int n_kv, int d, float scale, int causal, cudaStream_t st) {
-    if (total_q <= 0) return cudaSuccess;
-    const PromptArgs a{q, k, v, out, cu_q, cu_k, prefix, n_seq, total_q, total_k, n_q, n_kv, d, causal,
-                       scale * 1.4426950408889634f};
-    const dim3 grid((unsigned)((total_q + 3) / 4), (unsigned)n_q);
-    const cudaError_t e = type == kBF16 ? launch_k(prompt_row_kernel<__nv_bfloat16>, grid, dim3(128), 0, st, a)
-                          : type == kF16 ? launch_k(prompt_row_kernel<__half>, grid, dim3(128), 0, st, a)
-                                         : cudaErrorInvalidValue;
+    if (total_q <= 0 || n_seq <= 0) return cudaSuccess;
+    PromptArgs a{q, k, v, out, cu_q, cu_k, prefix, n_seq, total_q, total_k, n_q, n_kv, d, causal, scale < 0.f,
+                 fabsf(scale) * 1.4426950408889634f, 1, kPaRows};
+    if (a.scale_log2 < 1e-30f) a.scale_log2 = 1e-30f;   // scale 0: equal weights, but a masked score stays -inf
+    // the whole group shares a tile where that fills at least 120 of its 128
+    // rows, else the largest part of it that does (1 always does)
+    const int group = n_q / n_kv;
+    for (int g = 1; g <= group && g <= kPaRows; ++g)
+        if (group % g == 0 && kPaRows / g * g >= 120) a.gp = g;
+    a.tile_tok = kPaRows / a.gp;
+    cudaError_t e;
+    if (type == kBF16) e = d > 64 ? prompt_launch<__nv_bfloat16, 128>(a, st) : prompt_launch<__nv_bfloat16, 64>(a, st);
+    else if (type == kF16) e = d > 64 ? prompt_launch<__half, 128>(a, st) : prompt_launch<__half, 64>(a, st);
+    else return cudaErrorInvalidValue;
     return e != cudaSuccess ? e : cudaGetLastError();
 }
 

@@ -755,7 +755,7 @@ static bool heads_ok(int32_t n_q, int32_t n_kv) {
 static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 // a 16-bit operand that a tensor map can describe
 static bool tma_ok(const void* p, int64_t tok, int64_t head) {
-    return p && aligned16(p) && tok >= 0 && head >= 0 && tok % 8 == 0 && head % 8 == 0;
+    return p && aligned16(p) && tok > 0 && head > 0 && tok % 8 == 0 && head % 8 == 0;
 }
 
 int32_t vla_cuda_qk_norm_rope(void* q_out, void* k_out, int32_t out_type, const void* q, int64_t q_tok, int64_t q_head,

@@ -301,9 +301,9 @@ def qk_norm_rope(q, k, pos, sections, q_weight=None, k_weight=None, eps=1e-6, ba
 
 
 def _tma_heads(x, name):
-    """_heads whose address and strides are multiples of 16 bytes (a copy where they are not)."""
+    """_heads whose address and strides are (nonzero) multiples of 16 bytes; a copy where they are not."""
     x = _heads(x, name)
-    if x.data_ptr() % 16 or x.stride(0) % 8 or x.stride(1) % 8:
+    if x.data_ptr() % 16 or x.stride(0) % 8 or x.stride(1) % 8 or not x.stride(0) or not x.stride(1):
         x = x.clone(memory_format=torch.contiguous_format)
     return x
 
