@@ -8,7 +8,6 @@ memory and the stream handle only; the compute is the library's kernels.
 from __future__ import annotations
 
 import ctypes
-import math
 
 import torch
 
@@ -19,8 +18,14 @@ def _p(t):
     return None if t is None else t.data_ptr()
 
 
+# the current stream's handle alone: current_stream() builds a Stream object, 3 us a call
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    if _raw_stream is None:
+        return torch.cuda.current_stream().cuda_stream
+    return _raw_stream(torch.cuda.current_device())
 
 
 def i8_ld(K: int) -> int:
@@ -242,6 +247,9 @@ def conv_transpose1d(x, W, bias, k, stride, pad):
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 
+# A call of these takes a few microseconds on the device at single tokens, so the
+# wrappers look at each argument once.
+
 def _need(ok, what):
     if not ok:
         raise ValueError(what)
@@ -250,23 +258,39 @@ def _need(ok, what):
 def _on_device(*tensors):
     dev = torch.cuda.current_device()
     for t in tensors:
-        _need(t is None or (t.is_cuda and t.device.index == dev), "tensors have to be on the current CUDA device")
+        if t is not None and t.get_device() != dev:
+            raise ValueError("tensors have to be on the current CUDA device")
 
 
-def _typed(x, name):
-    _need(x.dtype in _TYPES, f"{name} has to be float32, float16 or bfloat16")
-    return _TYPES[x.dtype]
+def _typed(x):
+    t = _TYPES.get(x.dtype)
+    if t is None:
+        raise ValueError("q, k and v have to be float32, float16 or bfloat16")
+    return t
 
 
-def _heads(x, name):
-    """[tokens, heads, d] with contiguous channels; other strides stay as they are."""
-    _need(x.dim() == 3, f"{name} has to be [tokens, heads, head_dim]")
-    return x if x.stride(2) == 1 or x.shape[2] == 1 else x.contiguous()
+def _new(like, shape, dtype):
+    """A contiguous tensor for an output."""
+    if like.dtype is dtype and like.shape == shape and like.is_contiguous():
+        return torch.empty_like(like)
+    return like.new_empty(shape, dtype=dtype)
 
 
-def _int32(x, name):
-    _need(x.dtype == torch.int32, f"{name} has to be int32")
-    return x.contiguous()
+def _heads(x):
+    """[tokens, heads, d] with contiguous channels; other strides stay as they are. Returns it and its strides."""
+    if x.dim() != 3:
+        raise ValueError("q, k and v have to be [tokens, heads, head_dim]")
+    st = x.stride()
+    if st[2] != 1 and x.shape[2] != 1:
+        x = x.contiguous()
+        st = x.stride()
+    return x, st
+
+
+def _int32(x, what):
+    if x.dtype is not torch.int32:
+        raise ValueError(f"{what} has to be int32")
+    return x if x.is_contiguous() else x.contiguous()
 
 
 def qk_norm_rope(q, k, pos, sections, q_weight=None, k_weight=None, eps=1e-6, base=10000.0, restart=False,
@@ -275,61 +299,64 @@ def qk_norm_rope(q, k, pos, sections, q_weight=None, k_weight=None, eps=1e-6, ba
 
     q [T, n_q, d], k [T, n_kv, d] (or None); pos int32 [axes, T]; sections: rotated pairs of each axis; weights
     fp32 [d] or None (no norm). Returns (q_out, k_out) in out_dtype (default: q's)."""
-    q = _heads(q, "q")
+    q, qs = _heads(q)
     T, n_q, d = q.shape
-    in_type, out_dtype = _typed(q, "q"), out_dtype or q.dtype
+    in_type = _typed(q)
+    if out_dtype is None:
+        out_dtype = q.dtype
     _need(out_dtype in _TYPES, "out_dtype has to be float32, float16 or bfloat16")
-    n_kv, k_out = 0, None
+    n_kv, k_out, ks = 0, None, (0, 0)
     if k is not None:
-        k = _heads(k, "k")
-        _need(k.dtype == q.dtype and k.shape[0] == T and k.shape[2] == d, "k has to match q in type, tokens and width")
+        k, ks = _heads(k)
         n_kv = k.shape[1]
-        k_out = torch.empty((T, n_kv, d), dtype=out_dtype, device=q.device)
+        _need(k.dtype is q.dtype and k.shape[0] == T and k.shape[2] == d, "k has to match q in type, tokens and width")
+        k_out = _new(k, (T, n_kv, d), out_dtype)
+    axes = len(sections)
     pos = _int32(pos, "pos")
-    _need(tuple(pos.shape) == (len(sections), T), "pos has to be [axes, tokens], one axis for each of sections")
+    _need(pos.shape == (axes, T), "pos has to be [axes, tokens], one axis for each of sections")
     for w in (q_weight, k_weight):
-        _need(w is None or (w.dtype == torch.float32 and tuple(w.shape) == (d,) and w.is_contiguous()),
-              "weights have to be contiguous float32 [head_dim]")
+        if w is not None:
+            _need(w.dtype is torch.float32 and w.shape == (d,) and w.is_contiguous(),
+                  "weights have to be contiguous float32 [head_dim]")
     _on_device(q, k, pos, q_weight, k_weight)
-    q_out = torch.empty((T, n_q, d), dtype=out_dtype, device=q.device)
-    ks = (0, 0) if k is None else (k.stride(0), k.stride(1))
-    check(lib().vla_cuda_qk_norm_rope(_p(q_out), _p(k_out), _TYPES[out_dtype], _p(q), q.stride(0), q.stride(1), _p(k),
-                                      *ks, in_type, _p(pos), (ctypes.c_int32 * len(sections))(*sections),
-                                      len(sections), 1 if restart else 0, _p(q_weight), _p(k_weight), eps, base, T, n_q,
-                                      n_kv, d, _stream()), "vla_cuda_qk_norm_rope")
+    q_out = _new(q, (T, n_q, d), out_dtype)
+    check(lib().vla_cuda_qk_norm_rope(q_out.data_ptr(), _p(k_out), _TYPES[out_dtype], q.data_ptr(), qs[0], qs[1], _p(k),
+                                      ks[0], ks[1], in_type, pos.data_ptr(), (ctypes.c_int32 * axes)(*sections), axes,
+                                      restart, _p(q_weight), _p(k_weight), eps, base, T, n_q, n_kv, d, _stream()),
+          "vla_cuda_qk_norm_rope")
     return q_out, k_out
 
 
-def _tma_heads(x, name):
+def _tma_heads(x):
     """_heads whose address and strides are (nonzero) multiples of 16 bytes; a copy where they are not."""
-    x = _heads(x, name)
-    if x.data_ptr() % 16 or x.stride(0) % 8 or x.stride(1) % 8 or not x.stride(0) or not x.stride(1):
+    x, st = _heads(x)
+    if x.data_ptr() % 16 or st[0] % 8 or st[1] % 8 or not st[0] or not st[1]:
         x = x.clone(memory_format=torch.contiguous_format)
-    return x
+        st = x.stride()
+    return x, st
 
 
 def prompt_attention(q, k, v, cu_q, cu_k=None, scale=None, causal=True, prefix=None):
     """Attention over packed prompts: q [Tq, n_q, d], k / v [Tk, n_kv, d] (fp16 or bf16), cu_q / cu_k int32
     [n_seq + 1] (cu_k defaults to cu_q), prefix int32 [n_seq] or None. Returns [Tq, n_q, d]."""
-    q, k, v = _tma_heads(q, "q"), _tma_heads(k, "k"), _tma_heads(v, "v")
+    (q, qs), (k, ks), (v, vs) = _tma_heads(q), _tma_heads(k), _tma_heads(v)
     Tq, n_q, d = q.shape
-    Tk, n_kv = k.shape[:2]
-    _need(q.dtype in (torch.float16, torch.bfloat16) and k.dtype == q.dtype and v.dtype == q.dtype,
-          "q, k and v have to be float16, or bfloat16")
-    _need(k.shape == v.shape and k.shape[2] == d, "k and v have to match in shape, and q in width")
+    Tk, n_kv, dk = k.shape
+    typ = _typed(q)
+    _need(typ and k.dtype is q.dtype and v.dtype is q.dtype, "q, k and v have to be float16, or bfloat16")
+    _need(k.shape == v.shape and dk == d, "k and v have to match in shape, and q in width")
     cu_q = _int32(cu_q, "cu_q")
     cu_k = cu_q if cu_k is None else _int32(cu_k, "cu_k")
-    _need(cu_q.dim() == 1 and cu_q.shape == cu_k.shape and cu_q.numel() > 0, "cu_q and cu_k have to be [n_seq + 1]")
     n_seq = cu_q.numel() - 1
+    _need(cu_q.dim() == 1 and cu_q.shape == cu_k.shape and n_seq >= 0, "cu_q and cu_k have to be [n_seq + 1]")
     if prefix is not None:
         prefix = _int32(prefix, "prefix")
-        _need(tuple(prefix.shape) == (n_seq,), "prefix has to be [n_seq]")
+        _need(prefix.shape == (n_seq,), "prefix has to be [n_seq]")
     _on_device(q, k, v, cu_q, cu_k, prefix)
-    out = torch.empty((Tq, n_q, d), dtype=q.dtype, device=q.device)
-    check(lib().vla_cuda_prompt_attention(_p(out), _p(q), q.stride(0), q.stride(1), _p(k), k.stride(0), k.stride(1),
-                                          _p(v), v.stride(0), v.stride(1), _TYPES[q.dtype], _p(cu_q), _p(cu_k),
-                                          _p(prefix), n_seq, Tq, Tk, n_q, n_kv, d,
-                                          1.0 / math.sqrt(d) if scale is None else scale, 1 if causal else 0,
+    out = _new(q, (Tq, n_q, d), q.dtype)
+    check(lib().vla_cuda_prompt_attention(out.data_ptr(), q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1],
+                                          v.data_ptr(), vs[0], vs[1], typ, cu_q.data_ptr(), cu_k.data_ptr(), _p(prefix),
+                                          n_seq, Tq, Tk, n_q, n_kv, d, d ** -0.5 if scale is None else scale, causal,
                                           _stream()), "vla_cuda_prompt_attention")
     return out
 
@@ -342,38 +369,43 @@ def kv4_cache(n_pages, n_kv, head_dim, page=64, device="cuda"):
 
 
 def _cache(cache):
-    _need(cache.dtype == torch.uint8 and cache.dim() == 4 and cache.is_contiguous() and cache.shape[3] % 20 == 0,
-          "cache has to be kv4_cache's")
+    if cache.dtype is not torch.uint8 or cache.dim() != 4 or not cache.is_contiguous() or cache.shape[3] % 20:
+        raise ValueError("cache has to be kv4_cache's")
     n_pages, n_kv, blocks, size = cache.shape
     return n_pages, n_kv, 16 * blocks, size // 20
+
+
+def _slots(slots, T):
+    if slots.dtype is not torch.int64 or slots.dim() != 1 or (T is not None and slots.shape[0] != T):
+        raise ValueError("slots has to be int64 [tokens]")
+    return slots if slots.is_contiguous() else slots.contiguous()
 
 
 def kv4_append(cache, k, v, slots):
     """Quantizes k and v [T, n_kv, d] into the cache's slots (int64 [T], negative: skipped)."""
     n_pages, n_kv, page, d = _cache(cache)
-    k, v = _heads(k, "k"), _heads(v, "v")
+    (k, ks), (v, vs) = _heads(k), _heads(v)
     T = k.shape[0]
-    _need(tuple(k.shape) == (T, n_kv, d) and k.shape == v.shape and k.dtype == v.dtype,
+    _need(k.shape == (T, n_kv, d) and k.shape == v.shape and k.dtype is v.dtype,
           "k and v have to be [tokens, n_kv, head_dim] of the cache, of one type")
-    _need(slots.dtype == torch.int64 and tuple(slots.shape) == (T,), "slots has to be int64 [tokens]")
-    slots = slots.contiguous()
+    slots = _slots(slots, T)
     _on_device(cache, k, v, slots)
-    check(lib().vla_cuda_kv4_append(_p(cache), n_pages, page, _p(k), k.stride(0), k.stride(1), _p(v), v.stride(0),
-                                    v.stride(1), _typed(k, "k"), _p(slots), T, n_kv, d, _stream()),
-          "vla_cuda_kv4_append")
+    check(lib().vla_cuda_kv4_append(cache.data_ptr(), n_pages, page, k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0],
+                                    vs[1], _typed(k), slots.data_ptr(), T, n_kv, d, _stream()), "vla_cuda_kv4_append")
 
 
 def kv4_read(cache, slots, dtype=torch.float32):
     """The values of the cache's slots: (k, v) [T, n_kv, d]; zeros for a negative slot."""
     n_pages, n_kv, page, d = _cache(cache)
-    _need(dtype in _TYPES, "dtype has to be float32, float16 or bfloat16")
-    _need(slots.dtype == torch.int64 and slots.dim() == 1, "slots has to be int64 [tokens]")
-    slots = slots.contiguous()
+    typ = _TYPES.get(dtype)
+    _need(typ is not None, "dtype has to be float32, float16 or bfloat16")
+    slots = _slots(slots, None)
     _on_device(cache, slots)
-    k = torch.empty((slots.numel(), n_kv, d), dtype=dtype, device=cache.device)
+    T = slots.shape[0]
+    k = cache.new_empty((T, n_kv, d), dtype=dtype)
     v = torch.empty_like(k)
-    check(lib().vla_cuda_kv4_read(_p(cache), n_pages, page, _p(k), _p(v), _TYPES[dtype], _p(slots), slots.numel(), n_kv,
-                                  d, _stream()), "vla_cuda_kv4_read")
+    check(lib().vla_cuda_kv4_read(cache.data_ptr(), n_pages, page, k.data_ptr(), v.data_ptr(), typ, slots.data_ptr(), T,
+                                  n_kv, d, _stream()), "vla_cuda_kv4_read")
     return k, v
 
 
@@ -381,25 +413,32 @@ def kv4_attention(q, cache, table, lens, scale=None, causal=True):
     """Attention of new tokens over the 4-bit cache: q [B, n_q, d] or [B, queries, n_q, d], table int32 [B, pages],
     lens int32 [B] (tokens in the cache, the new ones among them). Returns q's shape and type."""
     n_pages, n_kv, page, d = _cache(cache)
-    _need(q.dim() in (3, 4) and q.shape[-1] == d, "q has to be [batch, (queries,) n_q, head_dim] of the cache's width")
-    x = q if q.stride(-1) == 1 else q.contiguous()
-    B, n_q = x.shape[0], x.shape[-2]
-    queries, q_tok = (1, 0) if x.dim() == 3 else (x.shape[1], x.stride(1))
-    typ = _typed(x, "q")
-    _need(table.dtype == torch.int32 and table.dim() == 2 and table.shape[0] == B, "table has to be int32 [batch, pages]")
-    if table.stride(1) != 1 or (B > 1 and table.stride(0) < table.shape[1]):
-        table = table.contiguous()
-    lens = _int32(lens, "lens")
-    _need(tuple(lens.shape) == (B,), "lens has to be [batch]")
-    _on_device(x, cache, table, lens)
-    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    shape = q.shape
+    _need(len(shape) in (3, 4) and shape[-1] == d, "q has to be [batch, (queries,) n_q, head_dim] of the cache's width")
+    st = q.stride()
+    if st[-1] != 1:
+        q = q.contiguous()
+        st = q.stride()
+    B, n_q = shape[0], shape[-2]
+    queries, q_tok = (1, 0) if len(shape) == 3 else (shape[1], st[1])
+    typ = _typed(q)
+    _need(table.dtype is torch.int32 and table.dim() == 2 and table.shape[0] == B, "table has to be int32 [batch, pages]")
     pages = table.shape[1]
-    size = int(lib().vla_cuda_kv4_attention_workspace_bytes(B, queries, n_q, n_kv, d, pages, page))
-    ws = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
-    check(lib().vla_cuda_kv4_attention(_p(out), _p(x), x.stride(0), q_tok, x.stride(-2), typ, _p(cache), n_pages, page,
-                                       _p(table), max(table.stride(0), pages), pages, _p(lens), B, queries, n_q, n_kv, d,
-                                       1.0 / math.sqrt(d) if scale is None else scale, 1 if causal else 0, _p(ws),
-                                       size, _stream()), "vla_cuda_kv4_attention")
+    ld, step = table.stride()
+    if step != 1 or ld < pages:
+        table = table.contiguous()
+        ld = pages
+    lens = _int32(lens, "lens")
+    _need(lens.shape == (B,), "lens has to be [batch]")
+    _on_device(q, cache, table, lens)
+    L = lib()
+    out = _new(q, shape, q.dtype)
+    size = L.vla_cuda_kv4_attention_workspace_bytes(B, queries, n_q, n_kv, d, pages, page)
+    ws = cache.new_empty(size) if size else None
+    check(L.vla_cuda_kv4_attention(out.data_ptr(), q.data_ptr(), st[0], q_tok, st[-2], typ, cache.data_ptr(), n_pages,
+                                   page, table.data_ptr(), ld, pages, lens.data_ptr(), B, queries, n_q, n_kv, d,
+                                   d ** -0.5 if scale is None else scale, causal, _p(ws), size, _stream()),
+          "vla_cuda_kv4_attention")
     return out
 
 
