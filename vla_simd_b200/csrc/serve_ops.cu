@@ -8,6 +8,9 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <algorithm>
+#include <climits>
+
 namespace vsb {
 
 namespace {
@@ -52,116 +55,107 @@ struct RopeArgs {
     void *q_out, *k_out;
     const int* pos;
     const float *qw, *kw;
-    float eps;
+    float eps, inv_d;
     int tokens, n_q, n_kv, d, rot;
+    int per_token;   // warps that share a token
     RopeTable tab;
 };
 
 constexpr int kRopeThreads = 256;
 
-// sin and cos of every pair of tokens [t0, t0 + nt) into shared memory
-__device__ __forceinline__ void rope_turns(const RopeArgs& a, int t0, int nt, float2* cs) {
-    const int pairs = a.rot / 2;
-    for (int i = threadIdx.x; i < nt * pairs; i += blockDim.x) {
-        const int t = i / pairs, p = i - t * pairs;
-        const double turn = (double)a.pos[(long long)a.tab.axis[p] * a.tokens + t0 + t] * a.tab.turns[p];
-        float s, c;
-        sincospif(2.0f * (float)(turn - rint(turn)), &s, &c);
-        cs[i] = make_float2(c, s);
-    }
+// cos and sin of the angle of a pair whose frequency is `turns` (in whole turns)
+__device__ __forceinline__ float2 rope_turn(int pos, double turns) {
+    const double turn = (double)pos * turns;
+    float s, c;
+    sincospif(2.0f * (float)(turn - rint(turn)), &s, &c);
+    return make_float2(c, s);
 }
 
-// A group of GS lanes (a power of two >= d / 8) owns a row; lane l holds the
-// two quads of channels [c0, c0 + 4) and [c1, c1 + 4) that pair up with each
-// other, so a row is rotated without exchanging values.
-template <typename TI, typename TO, int TT>
+// A warp has one token (or a share of its heads). GS lanes (the power of two >= d
+// / 8) have a row; lane l the two quads of channels [c0, c0 + 4) and [c1, c1 + 4)
+// that pair up with each other, so a row is rotated without exchanging values and
+// a lane's four sines and cosines, in registers, serve every head. kRows rows a
+// lane are loaded before the first is used.
+template <typename TI, typename TO>
 __global__ void __launch_bounds__(kRopeThreads)
 qk_norm_rope_kernel(const __grid_constant__ RopeArgs a, int gs) {
-    extern __shared__ float2 cs[];
-    const int t0 = blockIdx.x * TT, nt = min(TT, a.tokens - t0);
-    const int lane = threadIdx.x & (gs - 1), sub = threadIdx.x / gs, n_sub = kRopeThreads / gs;
-    const bool on = lane < a.d / 8;
-    const bool turned = lane < a.rot / 8;
-    const int c0 = turned ? 4 * lane : 8 * lane, c1 = turned ? a.rot / 2 + 4 * lane : 8 * lane + 4;
-    float4 wq[2], wk[2];
-    const float4 one = make_float4(1.f, 1.f, 1.f, 1.f);
-    wq[0] = wq[1] = wk[0] = wk[1] = one;
-    if (on && a.qw) {
-        wq[0] = *reinterpret_cast<const float4*>(a.qw + c0);
-        wq[1] = *reinterpret_cast<const float4*>(a.qw + c1);
+    __shared__ double turns[kMaxPairs];
+    __shared__ unsigned char axis[kMaxPairs];
+    const int wid = blockIdx.x * (kRopeThreads / 32) + (threadIdx.x >> 5);
+    const int t = wid / a.per_token, share = wid - t * a.per_token;
+    const int lane = threadIdx.x & (gs - 1), sub = (threadIdx.x & 31) / gs, n_sub = 32 / gs;
+    for (int i = threadIdx.x; i < a.rot / 2; i += kRopeThreads) {   // once a CTA: lanes index it apart
+        turns[i] = a.tab.turns[i];
+        axis[i] = a.tab.axis[i];
     }
-    if (on && a.kw) {
-        wk[0] = *reinterpret_cast<const float4*>(a.kw + c0);
-        wk[1] = *reinterpret_cast<const float4*>(a.kw + c1);
-    }
+    __syncthreads();
     pdl_trigger();
     pdl_wait();
-    rope_turns(a, t0, nt, cs);
-    __syncthreads();
-    const int nh = a.n_q + a.n_kv, rows = nt * nh;
+    if (t >= a.tokens) return;
+    const bool on = lane < a.d / 8, turned = lane < a.rot / 8;
+    const int c0 = turned ? 4 * lane : 8 * lane, c1 = turned ? a.rot / 2 + 4 * lane : 8 * lane + 4;
     using P = Pack<TI, 4>;
     using PO = Pack<TO, 4>;
-    constexpr int U = 4;   // rows in flight per lane group
-    for (int r0 = sub; r0 < rows; r0 += U * n_sub) {
-        P x[U][2];
-        #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int r = r0 + u * n_sub;
-            if (r < rows && on) {
-                const int t = r / nh, h = r - t * nh;
-                const TI* src = h < a.n_q
-                    ? static_cast<const TI*>(a.q.p) + (long long)(t0 + t) * a.q.tok + (long long)h * a.q.head
-                    : static_cast<const TI*>(a.k.p) + (long long)(t0 + t) * a.k.tok + (long long)(h - a.n_q) * a.k.head;
-                x[u][0] = *reinterpret_cast<const P*>(src + c0);
-                x[u][1] = *reinterpret_cast<const P*>(src + c1);
-            } else {
-                x[u][0] = x[u][1] = P{};
-            }
+    constexpr int kRows = 4;
+    float2 cs[4];
+    #pragma unroll
+    for (int e = 0; e < 4; ++e)
+        cs[e] = turned ? rope_turn(a.pos[(long long)axis[4 * lane + e] * a.tokens + t], turns[4 * lane + e])
+                       : make_float2(1.f, 0.f);
+    #pragma unroll 1
+    for (int part = 0; part < 2; ++part) {
+        const int nh = part ? a.n_kv : a.n_q;
+        const HeadsIn& in = part ? a.k : a.q;
+        const TI* src = static_cast<const TI*>(in.p) + (long long)t * in.tok;
+        TO* dst = static_cast<TO*>(part ? a.k_out : a.q_out) + (long long)t * nh * a.d;
+        const float* wp = part ? a.kw : a.qw;
+        float4 w0 = make_float4(1.f, 1.f, 1.f, 1.f), w1 = w0;
+        if (wp && on) {
+            w0 = *reinterpret_cast<const float4*>(wp + c0);
+            w1 = *reinterpret_cast<const float4*>(wp + c1);
         }
-        #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int r = r0 + u * n_sub;
-            const int t = r / nh, h = r - t * nh;
-            const bool isq = h < a.n_q;
-            float y0[4], y1[4];
-            float ss = 0.f;
+        for (int h0 = share * n_sub + sub; h0 - sub < nh; h0 += kRows * a.per_token * n_sub) {
+            P x[kRows][2];
             #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                y0[e] = to_f(x[u][0].v[e]);
-                y1[e] = to_f(x[u][1].v[e]);
-                ss = fmaf(y0[e], y0[e], ss);
-                ss = fmaf(y1[e], y1[e], ss);
+            for (int u = 0; u < kRows; ++u) {
+                const int h = h0 + u * a.per_token * n_sub;
+                x[u][0] = x[u][1] = P{};
+                if (h < nh && on) {
+                    x[u][0] = *reinterpret_cast<const P*>(src + (long long)h * in.head + c0);
+                    x[u][1] = *reinterpret_cast<const P*>(src + (long long)h * in.head + c1);
+                }
             }
-            const bool normed = isq ? a.qw != nullptr : a.kw != nullptr;
-            for (int o = gs >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-            if (r >= rows || !on) continue;
-            if (normed) {
-                const float inv = rsqrtf(ss / (float)a.d + a.eps);
-                const float4 w0 = isq ? wq[0] : wk[0], w1 = isq ? wq[1] : wk[1];
-                y0[0] *= inv * w0.x; y0[1] *= inv * w0.y; y0[2] *= inv * w0.z; y0[3] *= inv * w0.w;
-                y1[0] *= inv * w1.x; y1[1] *= inv * w1.y; y1[2] *= inv * w1.z; y1[3] *= inv * w1.w;
-            }
-            if (turned) {
-                const float4* c4 = reinterpret_cast<const float4*>(cs + t * (a.rot / 2) + 4 * lane);
-                const float4 ca = c4[0], cb = c4[1];   // (cos, sin) of two pairs each
-                const float co[4] = {ca.x, ca.z, cb.x, cb.z}, si[4] = {ca.y, ca.w, cb.y, cb.w};
+            #pragma unroll
+            for (int u = 0; u < kRows; ++u) {
+                const int h = h0 + u * a.per_token * n_sub;
+                if (h - sub >= nh) break;   // the same for the whole warp
+                float y0[4], y1[4];
+                #pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    y0[e] = to_f(x[u][0].v[e]);
+                    y1[e] = to_f(x[u][1].v[e]);
+                }
+                if (wp) {
+                    float ss = 0.f;
+                    #pragma unroll
+                    for (int e = 0; e < 4; ++e) ss = fmaf(y0[e], y0[e], fmaf(y1[e], y1[e], ss));
+                    for (int o = gs >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+                    const float inv = rsqrtf(fmaf(ss, a.inv_d, a.eps));
+                    y0[0] *= inv * w0.x; y0[1] *= inv * w0.y; y0[2] *= inv * w0.z; y0[3] *= inv * w0.w;
+                    y1[0] *= inv * w1.x; y1[1] *= inv * w1.y; y1[2] *= inv * w1.z; y1[3] *= inv * w1.w;
+                }
+                PO o0, o1;
                 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const float u0 = y0[e], u1 = y1[e];
-                    y0[e] = fmaf(u0, co[e], -(u1 * si[e]));
-                    y1[e] = fmaf(u1, co[e], u0 * si[e]);
+                    o0.v[e] = from_f<TO>(turned ? fmaf(u0, cs[e].x, -(u1 * cs[e].y)) : u0);
+                    o1.v[e] = from_f<TO>(turned ? fmaf(u1, cs[e].x, u0 * cs[e].y) : u1);
+                }
+                if (h < nh && on) {
+                    *reinterpret_cast<PO*>(dst + (long long)h * a.d + c0) = o0;
+                    *reinterpret_cast<PO*>(dst + (long long)h * a.d + c1) = o1;
                 }
             }
-            TO* dst = isq ? static_cast<TO*>(a.q_out) + ((long long)(t0 + t) * a.n_q + h) * a.d
-                          : static_cast<TO*>(a.k_out) + ((long long)(t0 + t) * a.n_kv + (h - a.n_q)) * a.d;
-            PO o0, o1;
-            #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                o0.v[e] = from_f<TO>(y0[e]);
-                o1.v[e] = from_f<TO>(y1[e]);
-            }
-            *reinterpret_cast<PO*>(dst + c0) = o0;
-            *reinterpret_cast<PO*>(dst + c1) = o1;
         }
     }
 }
@@ -175,9 +169,10 @@ qk_norm_rope_any_kernel(const __grid_constant__ RopeArgs a) {
     const int t0 = blockIdx.x, lane = threadIdx.x & 31;
     pdl_trigger();
     pdl_wait();
-    rope_turns(a, t0, 1, cs);
-    __syncthreads();
     const int nh = a.n_q + a.n_kv, pairs = a.rot / 2;
+    for (int p = threadIdx.x; p < pairs; p += kRopeThreads)
+        cs[p] = rope_turn(a.pos[(long long)a.tab.axis[p] * a.tokens + t0], a.tab.turns[p]);
+    __syncthreads();
     for (int h = threadIdx.x >> 5; h < nh; h += kRopeThreads / 32) {
         const bool isq = h < a.n_q;
         const TI* src = isq ? static_cast<const TI*>(a.q.p) + (long long)t0 * a.q.tok + (long long)h * a.q.head
@@ -193,7 +188,7 @@ qk_norm_rope_any_kernel(const __grid_constant__ RopeArgs a) {
                 ss = fmaf(v, v, ss);
             }
             for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-            inv = rsqrtf(ss / (float)a.d + a.eps);
+            inv = rsqrtf(fmaf(ss, a.inv_d, a.eps));
         }
         for (int p = lane; p < pairs; p += 32) {
             float u0 = to_f(src[p]), u1 = to_f(src[p + pairs]);
@@ -224,7 +219,7 @@ cudaError_t qk_norm_rope(void* q_out, void* k_out, int out_type, const HeadsIn& 
                          const int* pos, const RopeTable& tab, int rot, const float* qw, const float* kw, float eps,
                          int tokens, int n_q, int n_kv, int d, cudaStream_t st) {
     if (tokens <= 0) return cudaSuccess;
-    RopeArgs a{q, k, q_out, k_out, pos, qw, kw, eps, tokens, n_q, n_kv, d, rot, tab};
+    RopeArgs a{q, k, q_out, k_out, pos, qw, kw, eps, 1.0f / (float)d, tokens, n_q, n_kv, d, rot, 1, tab};
     const size_t os = type_size(out_type);
     const bool quads = d % 8 == 0 && rot % 8 == 0 && heads_aligned(q, type_size(in_type), 4) &&
                        (n_kv == 0 || heads_aligned(k, type_size(in_type), 4)) &&
@@ -232,6 +227,12 @@ cudaError_t qk_norm_rope(void* q_out, void* k_out, int out_type, const HeadsIn& 
                        (reinterpret_cast<uintptr_t>(qw) | reinterpret_cast<uintptr_t>(kw)) % 16 == 0;
     int gs = 1;
     while (gs < d / 8) gs *= 2;
+    // few tokens: their heads are shared out, down to one round of rows a warp,
+    // until the warps fill the SMs
+    const int rounds = (std::max(n_q, n_kv) * gs + 31) / 32;
+    while (a.per_token < rounds && (long long)tokens * a.per_token < 148 * 16) a.per_token *= 2;
+    const long long warps = (long long)tokens * a.per_token;
+    if (warps > INT_MAX) return cudaErrorInvalidValue;
     const cudaError_t e = by_type(in_type, [&](auto ti) {
         return by_type(out_type, [&](auto to) {
             using TI = decltype(ti);
@@ -239,11 +240,8 @@ cudaError_t qk_norm_rope(void* q_out, void* k_out, int out_type, const HeadsIn& 
             if (!quads)
                 return launch_k(qk_norm_rope_any_kernel<TI, TO>, dim3(tokens), dim3(kRopeThreads),
                                 sizeof(float2) * (rot / 2), st, a);
-            if (tokens >= 2048)
-                return launch_k(qk_norm_rope_kernel<TI, TO, 4>, dim3((tokens + 3) / 4), dim3(kRopeThreads),
-                                sizeof(float2) * 4 * (rot / 2), st, a, gs);
-            return launch_k(qk_norm_rope_kernel<TI, TO, 1>, dim3(tokens), dim3(kRopeThreads),
-                            sizeof(float2) * (rot / 2), st, a, gs);
+            return launch_k(qk_norm_rope_kernel<TI, TO>, dim3((unsigned)((warps + 7) / 8)), dim3(kRopeThreads), 0, st, a,
+                            gs);
         });
     });
     return e != cudaSuccess ? e : cudaGetLastError();
@@ -278,9 +276,10 @@ struct Kv4At {
 // group g and quad that a lane handles
 __device__ __forceinline__ Kv4At kv4_at(const Kv4Cache& c, long long slot, int head, int g, int quad) {
     const int ng = c.d / kKv4Group;
-    const long long page = slot / c.page;
-    const int in_page = (int)(slot - page * c.page), blk = in_page / kKv4Block, t = in_page % kKv4Block;
-    uint8_t* b = c.p + ((page * c.n_kv + head) * (c.page / kKv4Block) + blk) * (20ll * c.d);
+    // pages are powers of two of at least a block, and at most 2^31 slots in all
+    const int shift = 31 - __clz(c.page), page = (int)slot >> shift;
+    const int blk = ((int)slot & (c.page - 1)) / kKv4Block, t = (int)slot % kKv4Block;
+    uint8_t* b = c.p + ((((long long)page * c.n_kv + head) << (shift - 4)) + blk) * (20ll * c.d);
     const int j = t >> 3;
     const int by_quad = ((((t & 7) >> 1) * ng + g) * 2 + j) * 2 + (t & 1);
     Kv4At r;
@@ -294,35 +293,62 @@ __device__ __forceinline__ Kv4At kv4_at(const Kv4Cache& c, long long slot, int h
     return r;
 }
 
+__device__ __forceinline__ float min_nan(float a, float b) {   // NaN if either is
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
 // codes of 8 channels (one nibble each) and the group's s, m; the group is
-// spread over the 4 lanes of a quad
+// spread over the 4 lanes of a quad. The quotient (x - m) / s is first taken as
+// a product with 1 / (15 s), saturated to [0, 1]: good to 2^-20 of a step. Only
+// where that leaves the nearest code open (a step's middle within 2^-16: one
+// group in 500 of random values) is it divided.
 __device__ __forceinline__ uint32_t kv4_quantize(const float (&x)[8], __half& s, __half& m) {
     float lo = x[0], hi = x[0];
-    bool bad = false;
     #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        lo = fminf(lo, x[i]);
-        hi = fmaxf(hi, x[i]);
-        bad |= !(fabsf(x[i]) <= 3.402823466e38f);
+    for (int i = 1; i < 8; ++i) {
+        lo = min_nan(lo, x[i]);
+        hi = max_nan(hi, x[i]);
     }
     #pragma unroll
     for (int o = 1; o < 4; o <<= 1) {
-        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-        bad |= __shfl_xor_sync(0xffffffffu, (int)bad, o) != 0;
+        lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+        hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
     }
+    const bool bad = !(fmaxf(fabsf(lo), fabsf(hi)) <= 3.402823466e38f) || lo != lo;
     lo = fminf(fmaxf(lo, -65504.0f), 65504.0f);
     hi = fminf(fmaxf(hi, -65504.0f), 65504.0f);
     s = __float2half_rn(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f));
     m = __float2half_rn(lo);
     if (bad) s = m = __ushort_as_half(0x7fff);
     const float sf = __half2float(s), mf = __half2float(m);
+    const float inv = sf > 0.0f ? __fdividef(1.0f, 15.0f * sf) : 0.0f;
+    // the code in the low bits of 1.5 * 2^23 + code
     uint32_t w = 0;
+    float nearest = 0.f;   // the largest distance of a quotient from its code
     #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        float c = sf > 0.0f ? rintf(__fdiv_rn(__fsub_rn(x[i], mf), sf)) : 0.0f;
-        c = fminf(fmaxf(c, 0.0f), 15.0f);
-        w |= (uint32_t)(int)c << (4 * i);
+        const float f = __saturatef(__fsub_rn(x[i], mf) * inv);
+        const float u = fmaf(f, 15.0f, kRoundConst);
+        nearest = fmaxf(nearest, fabsf(fmaf(f, 15.0f, kRoundConst - u)));
+        w += (__float_as_uint(u) - 0x4B400000u) << (4 * i);
+    }
+    if (nearest > 0.5f - 1.0f / 65536.0f) {
+        w = 0;
+        #pragma unroll 1
+        for (int i = 0; i < 8; ++i) {
+            float xi = x[0];
+            #pragma unroll
+            for (int y = 1; y < 8; ++y) xi = i == y ? x[y] : xi;
+            const float c = sf > 0.0f ? rintf(__fdiv_rn(__fsub_rn(xi, mf), sf)) : 0.0f;
+            w |= (uint32_t)(int)fminf(fmaxf(c, 0.0f), 15.0f) << (4 * i);
+        }
     }
     return w;
 }
@@ -366,10 +392,9 @@ __global__ void __launch_bounds__(kKv4Threads)
 kv4_append_kernel(Kv4Cache c, HeadsIn k, HeadsIn v, const long long* slots, int tokens, int vec) {
     pdl_trigger();
     pdl_wait();
-    const int lpr = c.d / 8;
-    const long long i = (long long)blockIdx.x * kKv4Threads + threadIdx.x;
-    const long long row = i / lpr;
-    const int l = (int)(i - row * lpr), head = blockIdx.y;
+    const int lanes = c.d == 128 ? 4 : 3;   // log2 of a row's
+    const long long row = ((long long)blockIdx.x * kKv4Threads + threadIdx.x) >> lanes;
+    const int l = threadIdx.x & ((1 << lanes) - 1), head = blockIdx.y;
     const bool on = row < tokens;
     const long long slot = on ? slots[row] : -1;
     const bool in = slot >= 0 && slot < c.n_pages * c.page;
@@ -403,10 +428,9 @@ __global__ void __launch_bounds__(kKv4Threads)
 kv4_read_kernel(Kv4Cache c, T* k_out, T* v_out, const long long* slots, int tokens) {
     pdl_trigger();
     pdl_wait();
-    const int lpr = c.d / 8;
-    const long long i = (long long)blockIdx.x * kKv4Threads + threadIdx.x;
-    const long long row = i / lpr;
-    const int l = (int)(i - row * lpr), head = blockIdx.y;
+    const int lanes = c.d == 128 ? 4 : 3;   // log2 of a row's
+    const long long row = ((long long)blockIdx.x * kKv4Threads + threadIdx.x) >> lanes;
+    const int l = threadIdx.x & ((1 << lanes) - 1), head = blockIdx.y;
     if (row >= tokens) return;
     const long long slot = slots[row];
     float x[8] = {};
