@@ -151,17 +151,6 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     return d;
 }
 
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi);
-template <>
-__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
-    uint32_t r;
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
-}
-template <>
-__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) { return pack_h2(lo, hi); }
-
 // What a CTA works on: tile t has rows of queries [tok[t], tok[t] + n_tok[t])
 // of the sequence and sees the first keys[t] of its lk keys.
 struct PromptJob {

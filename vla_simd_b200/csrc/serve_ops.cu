@@ -71,13 +71,81 @@ __device__ __forceinline__ float2 rope_turn(int pos, double turns) {
     return make_float2(c, s);
 }
 
+// four elements as two pairs of floats
+__device__ __forceinline__ void load_quad(const float* p, float2 (&x)[2]) {
+    const float4 v = *reinterpret_cast<const float4*>(p);
+    x[0] = make_float2(v.x, v.y);
+    x[1] = make_float2(v.z, v.w);
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ float2 unpack2(uint32_t w, __nv_bfloat16) {
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+}
+__device__ __forceinline__ float2 unpack2(uint32_t w, __half) {
+    return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+template <typename T>
+struct Quad {   // 16-bit
+    uint2 w;
+    __device__ __forceinline__ float2 lo() const { return unpack2(w.x, T{}); }
+    __device__ __forceinline__ float2 hi() const { return unpack2(w.y, T{}); }
+    __device__ __forceinline__ static Quad of(float2 a, float2 b) {
+        Quad q;
+        q.w = make_uint2(pack2<T>(a.x, a.y), pack2<T>(b.x, b.y));
+        return q;
+    }
+};
+template <>
+struct Quad<float> {
+    float4 w;
+    __device__ __forceinline__ float2 lo() const { return make_float2(w.x, w.y); }
+    __device__ __forceinline__ float2 hi() const { return make_float2(w.z, w.w); }
+    __device__ __forceinline__ static Quad of(float2 a, float2 b) {
+        Quad q;
+        q.w = make_float4(a.x, a.y, b.x, b.y);
+        return q;
+    }
+};
+
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;"
+        : "=l"(reinterpret_cast<unsigned long long&>(d))
+        : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)),
+          "l"(reinterpret_cast<unsigned long long&>(c)));
+    return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 d;
+    asm("mul.rn.f32x2 %0, %1, %2;"
+        : "=l"(reinterpret_cast<unsigned long long&>(d))
+        : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
+    return d;
+}
+
 // A warp has one token (or a share of its heads). GS lanes (the power of two >= d
 // / 8) have a row; lane l the two quads of channels [c0, c0 + 4) and [c1, c1 + 4)
 // that pair up with each other, so a row is rotated without exchanging values and
-// a lane's four sines and cosines, in registers, serve every head. kRows rows a
-// lane are loaded before the first is used.
-template <typename TI, typename TO>
-__global__ void __launch_bounds__(kRopeThreads)
+// a lane's four sines and cosines, times the norm's weights, serve every head
+// from registers: inv * (x0 (w0 cos) - x1 (w1 sin)). Two channels an instruction
+// (f32x2): at one instruction a channel the kernel was bound by issue (190 a row,
+// 32 us at 4099 tokens of 40 heads of 128). kRows rows a lane are loaded before
+// the first is used.
+template <typename TI, typename TO, bool FULL>   // FULL: every channel turns
+__global__ void __launch_bounds__(kRopeThreads, 4)
 qk_norm_rope_kernel(const __grid_constant__ RopeArgs a, int gs) {
     __shared__ double turns[kMaxPairs];
     __shared__ unsigned char axis[kMaxPairs];
@@ -92,69 +160,81 @@ qk_norm_rope_kernel(const __grid_constant__ RopeArgs a, int gs) {
     pdl_trigger();
     pdl_wait();
     if (t >= a.tokens) return;
-    const bool on = lane < a.d / 8, turned = lane < a.rot / 8;
+    const bool on = lane < a.d / 8, turned = FULL || lane < a.rot / 8;
     const int c0 = turned ? 4 * lane : 8 * lane, c1 = turned ? a.rot / 2 + 4 * lane : 8 * lane + 4;
-    using P = Pack<TI, 4>;
-    using PO = Pack<TO, 4>;
-    constexpr int kRows = 4;
-    float2 cs[4];
+    constexpr int kRows = sizeof(TI) == 4 ? 3 : 4;
+    float2 co[2], si[2];
     #pragma unroll
-    for (int e = 0; e < 4; ++e)
-        cs[e] = turned ? rope_turn(a.pos[(long long)axis[4 * lane + e] * a.tokens + t], turns[4 * lane + e])
-                       : make_float2(1.f, 0.f);
+    for (int e = 0; e < 4; ++e) {
+        const float2 v = turned && on ? rope_turn(a.pos[(long long)axis[4 * lane + e] * a.tokens + t], turns[4 * lane + e])
+                                      : make_float2(1.f, 0.f);
+        (e & 1 ? co[e >> 1].y : co[e >> 1].x) = v.x;
+        (e & 1 ? si[e >> 1].y : si[e >> 1].x) = v.y;
+    }
+    const int step = a.per_token * n_sub;
     #pragma unroll 1
     for (int part = 0; part < 2; ++part) {
         const int nh = part ? a.n_kv : a.n_q;
         const HeadsIn& in = part ? a.k : a.q;
-        const TI* src = static_cast<const TI*>(in.p) + (long long)t * in.tok;
-        TO* dst = static_cast<TO*>(part ? a.k_out : a.q_out) + (long long)t * nh * a.d;
+        const int first = share * n_sub + sub;
+        const TI* src = static_cast<const TI*>(in.p) + (long long)t * in.tok + (long long)first * in.head;
+        TO* dst = static_cast<TO*>(part ? a.k_out : a.q_out) + ((long long)t * nh + first) * a.d;
+        const long long src_step = step * in.head;
+        const int dst_step = step * a.d;
         const float* wp = part ? a.kw : a.qw;
-        float4 w0 = make_float4(1.f, 1.f, 1.f, 1.f), w1 = w0;
+        float2 w0[2], w1[2];
+        w0[0] = w0[1] = w1[0] = w1[1] = make_float2(1.f, 1.f);
         if (wp && on) {
-            w0 = *reinterpret_cast<const float4*>(wp + c0);
-            w1 = *reinterpret_cast<const float4*>(wp + c1);
+            load_quad(wp + c0, w0);
+            load_quad(wp + c1, w1);
         }
-        for (int h0 = share * n_sub + sub; h0 - sub < nh; h0 += kRows * a.per_token * n_sub) {
-            P x[kRows][2];
+        // x0 -> x0 * f00 - x1 * f01, x1 -> x1 * f11 + x0 * f10
+        float2 f00[2], f01[2], f10[2], f11[2];
+        #pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            f00[e] = mul2(w0[e], co[e]);
+            f01[e] = mul2(w1[e], make_float2(-si[e].x, -si[e].y));
+            f10[e] = mul2(w0[e], si[e]);
+            f11[e] = mul2(w1[e], co[e]);
+        }
+        for (int h0 = first; h0 - sub < nh; h0 += kRows * step) {
+            Quad<TI> x[kRows][2];
             #pragma unroll
             for (int u = 0; u < kRows; ++u) {
-                const int h = h0 + u * a.per_token * n_sub;
-                x[u][0] = x[u][1] = P{};
-                if (h < nh && on) {
-                    x[u][0] = *reinterpret_cast<const P*>(src + (long long)h * in.head + c0);
-                    x[u][1] = *reinterpret_cast<const P*>(src + (long long)h * in.head + c1);
+                x[u][0] = x[u][1] = Quad<TI>{};
+                if (h0 + u * step < nh && on) {
+                    x[u][0] = *reinterpret_cast<const Quad<TI>*>(src + c0);
+                    x[u][1] = *reinterpret_cast<const Quad<TI>*>(src + c1);
                 }
+                src += src_step;
             }
             #pragma unroll
             for (int u = 0; u < kRows; ++u) {
-                const int h = h0 + u * a.per_token * n_sub;
-                if (h - sub >= nh) break;   // the same for the whole warp
-                float y0[4], y1[4];
-                #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    y0[e] = to_f(x[u][0].v[e]);
-                    y1[e] = to_f(x[u][1].v[e]);
-                }
+                if (h0 - sub + u * step >= nh) break;   // the same for the whole warp
+                const float2 y0[2] = {x[u][0].lo(), x[u][0].hi()}, y1[2] = {x[u][1].lo(), x[u][1].hi()};
+                float2 inv2 = make_float2(1.f, 1.f);
                 if (wp) {
-                    float ss = 0.f;
-                    #pragma unroll
-                    for (int e = 0; e < 4; ++e) ss = fmaf(y0[e], y0[e], fmaf(y1[e], y1[e], ss));
+                    const float2 s2 = fma2(y0[0], y0[0], fma2(y0[1], y0[1], fma2(y1[0], y1[0], mul2(y1[1], y1[1]))));
+                    float ss = s2.x + s2.y;
                     for (int o = gs >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-                    const float inv = rsqrtf(fmaf(ss, a.inv_d, a.eps));
-                    y0[0] *= inv * w0.x; y0[1] *= inv * w0.y; y0[2] *= inv * w0.z; y0[3] *= inv * w0.w;
-                    y1[0] *= inv * w1.x; y1[1] *= inv * w1.y; y1[2] *= inv * w1.z; y1[3] *= inv * w1.w;
+                    inv2.x = inv2.y = rsqrtf(fmaf(ss, a.inv_d, a.eps));
                 }
-                PO o0, o1;
+                float2 r0[2], r1[2];
                 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float u0 = y0[e], u1 = y1[e];
-                    o0.v[e] = from_f<TO>(turned ? fmaf(u0, cs[e].x, -(u1 * cs[e].y)) : u0);
-                    o1.v[e] = from_f<TO>(turned ? fmaf(u1, cs[e].x, u0 * cs[e].y) : u1);
+                for (int e = 0; e < 2; ++e) {
+                    if (FULL || turned) {
+                        r0[e] = mul2(fma2(y0[e], f00[e], mul2(y1[e], f01[e])), inv2);
+                        r1[e] = mul2(fma2(y1[e], f11[e], mul2(y0[e], f10[e])), inv2);
+                    } else {
+                        r0[e] = mul2(mul2(y0[e], w0[e]), inv2);
+                        r1[e] = mul2(mul2(y1[e], w1[e]), inv2);
+                    }
                 }
-                if (h < nh && on) {
-                    *reinterpret_cast<PO*>(dst + (long long)h * a.d + c0) = o0;
-                    *reinterpret_cast<PO*>(dst + (long long)h * a.d + c1) = o1;
+                if (h0 + u * step < nh && on) {
+                    *reinterpret_cast<Quad<TO>*>(dst + c0) = Quad<TO>::of(r0[0], r0[1]);
+                    *reinterpret_cast<Quad<TO>*>(dst + c1) = Quad<TO>::of(r1[0], r1[1]);
                 }
+                dst += dst_step;
             }
         }
     }
@@ -240,8 +320,9 @@ cudaError_t qk_norm_rope(void* q_out, void* k_out, int out_type, const HeadsIn& 
             if (!quads)
                 return launch_k(qk_norm_rope_any_kernel<TI, TO>, dim3(tokens), dim3(kRopeThreads),
                                 sizeof(float2) * (rot / 2), st, a);
-            return launch_k(qk_norm_rope_kernel<TI, TO>, dim3((unsigned)((warps + 7) / 8)), dim3(kRopeThreads), 0, st, a,
-                            gs);
+            const dim3 grid((unsigned)((warps + 7) / 8));
+            return rot == d ? launch_k(qk_norm_rope_kernel<TI, TO, true>, grid, dim3(kRopeThreads), 0, st, a, gs)
+                            : launch_k(qk_norm_rope_kernel<TI, TO, false>, grid, dim3(kRopeThreads), 0, st, a, gs);
         });
     });
     return e != cudaSuccess ? e : cudaGetLastError();
@@ -266,31 +347,38 @@ cudaError_t qk_norm_rope(void* q_out, void* k_out, int out_type, const HeadsIn& 
 //   value scales [quad][g][j][e]  fp16
 //   value minima [quad][g][j][e]  fp16
 struct Kv4At {
-    uint32_t* kc;
-    __half *ks, *km;
-    uint16_t* vc;
-    __half *vs, *vm;
+    uint8_t* block;
+    int t;         // token in the block
+    int by_quad;   // index of its scale for this lane's group
 };
 
-// the block of slot (page, head), and the offsets of token t inside it for the
-// group g and quad that a lane handles
-__device__ __forceinline__ Kv4At kv4_at(const Kv4Cache& c, long long slot, int head, int g, int quad) {
-    const int ng = c.d / kKv4Group;
+__device__ __forceinline__ Kv4At kv4_at(const Kv4Cache& c, long long slot, int head, int ng, int g) {
     // pages are powers of two of at least a block, and at most 2^31 slots in all
-    const int shift = 31 - __clz(c.page), page = (int)slot >> shift;
-    const int blk = ((int)slot & (c.page - 1)) / kKv4Block, t = (int)slot % kKv4Block;
-    uint8_t* b = c.p + ((((long long)page * c.n_kv + head) << (shift - 4)) + blk) * (20ll * c.d);
-    const int j = t >> 3;
-    const int by_quad = ((((t & 7) >> 1) * ng + g) * 2 + j) * 2 + (t & 1);
+    const int shift = 31 - __clz(c.page), s = (int)slot;
+    const int blk = (s & (c.page - 1)) / kKv4Block;
     Kv4At r;
-    r.kc = reinterpret_cast<uint32_t*>(b) + (((j * 8 + (t & 7)) * 4 + quad) * ng + g);
-    r.ks = reinterpret_cast<__half*>(b + 8 * c.d) + by_quad;
-    r.km = reinterpret_cast<__half*>(b + 9 * c.d) + (((t & 7) * 2 + j) * ng + g);
-    // n = 2 quad and 2 quad + 1: the second at + 4 * ng words
-    r.vc = reinterpret_cast<uint16_t*>(b + 10 * c.d) + (((j * 8 + 2 * quad) * 4 + ((t & 7) >> 1)) * ng + g) * 2 + (t & 1);
-    r.vs = reinterpret_cast<__half*>(b + 18 * c.d) + by_quad;
-    r.vm = reinterpret_cast<__half*>(b + 19 * c.d) + by_quad;
+    r.t = s % kKv4Block;
+    r.block = c.p + ((((long long)(s >> shift) * c.n_kv + head) << (shift - 4)) + blk) * (20ll * c.d);
+    r.by_quad = ((((r.t & 7) >> 1) * ng + g) * 2 + (r.t >> 3)) * 2 + (r.t & 1);
     return r;
+}
+
+// where a lane's 8 channels 32 g + 8 quad + i lie: a word of key codes; the
+// halves of two words of value codes (channels 4 (2 quad) .. and 4 (2 quad + 1) ..),
+// 4 ng words apart
+__device__ __forceinline__ uint32_t* kv4_key_code(const Kv4At& at, int ng, int g, int quad) {
+    return reinterpret_cast<uint32_t*>(at.block) + (at.t * 4 + quad) * ng + g;
+}
+__device__ __forceinline__ uint16_t* kv4_value_code(const Kv4At& at, int ng, int g, int quad) {
+    return reinterpret_cast<uint16_t*>(at.block + 320 * ng) +
+           ((((at.t >> 3) * 8 + 2 * quad) * 4 + ((at.t & 7) >> 1)) * ng + g) * 2 + (at.t & 1);
+}
+__device__ __forceinline__ __half* kv4_key_min(const Kv4At& at, int ng, int g) {
+    return reinterpret_cast<__half*>(at.block + 288 * ng) + ((at.t & 7) * 2 + (at.t >> 3)) * ng + g;
+}
+// scales of the keys at byte 256 ng, of the values at 576 ng, minima of the values at 608 ng
+__device__ __forceinline__ __half* kv4_by_quad(const Kv4At& at, int byte) {
+    return reinterpret_cast<__half*>(at.block + byte) + at.by_quad;
 }
 
 __device__ __forceinline__ float min_nan(float a, float b) {   // NaN if either is
@@ -383,67 +471,66 @@ __device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
     }
 }
 
-// One lane = 8 channels of one token, head and of keys or values; d / 8 lanes a
-// row. Rows run over the tokens first, so that a warp writes both halves of a
-// value word and whole sectors of codes when neighbouring tokens have
+// One lane = 8 channels of the key and of the value of one token and head; 4 NG
+// lanes a row. Rows run over the tokens first, so that a warp writes both halves
+// of a value word and whole sectors of codes when neighbouring tokens have
 // neighbouring slots.
-template <typename T>
+template <typename T, int NG>
 __global__ void __launch_bounds__(kKv4Threads)
 kv4_append_kernel(Kv4Cache c, HeadsIn k, HeadsIn v, const long long* slots, int tokens, int vec) {
     pdl_trigger();
     pdl_wait();
-    const int lanes = c.d == 128 ? 4 : 3;   // log2 of a row's
-    const long long row = ((long long)blockIdx.x * kKv4Threads + threadIdx.x) >> lanes;
-    const int l = threadIdx.x & ((1 << lanes) - 1), head = blockIdx.y;
+    const long long row = ((long long)blockIdx.x * kKv4Threads + threadIdx.x) / (4 * NG);
+    const int l = threadIdx.x % (4 * NG), g = l >> 2, quad = l & 3, head = blockIdx.y;
     const bool on = row < tokens;
     const long long slot = on ? slots[row] : -1;
     const bool in = slot >= 0 && slot < c.n_pages * c.page;
     if (on && slot >= c.n_pages * c.page) record_status(kStatusBadShape);
-    const T* src = blockIdx.z ? static_cast<const T*>(v.p) + row * v.tok + head * v.head
-                              : static_cast<const T*>(k.p) + row * k.tok + head * k.head;
-    float x[8] = {};
-    if (in) load8(src + 8 * l, vec, x);
-    __half s, m;
-    const uint32_t w = kv4_quantize(x, s, m);
-    if (!in) return;
-    const Kv4At at = kv4_at(c, slot, head, l >> 2, l & 3);
-    if (blockIdx.z == 0) {
-        *at.kc = w;
-        if ((l & 3) == 0) {
-            *at.ks = s;
-            *at.km = m;
-        }
-    } else {
-        at.vc[0] = (uint16_t)w;
-        at.vc[4 * (c.d / kKv4Group) * 2] = (uint16_t)(w >> 16);
-        if ((l & 3) == 0) {
-            *at.vs = s;
-            *at.vm = m;
-        }
+    float xk[8] = {}, xv[8] = {};
+    if (on) {   // not waiting for the slot
+        load8(static_cast<const T*>(k.p) + row * k.tok + head * k.head + 8 * l, vec, xk);
+        load8(static_cast<const T*>(v.p) + row * v.tok + head * v.head + 8 * l, vec, xv);
     }
+    __half ks, km, vs, vm;
+    const uint32_t wk = kv4_quantize(xk, ks, km), wv = kv4_quantize(xv, vs, vm);
+    if (!in) return;
+    const Kv4At at = kv4_at(c, slot, head, NG, g);
+    *kv4_key_code(at, NG, g, quad) = wk;
+    uint16_t* vc = kv4_value_code(at, NG, g, quad);
+    vc[0] = (uint16_t)wv;
+    vc[8 * NG] = (uint16_t)(wv >> 16);
+    // one lane of the group writes each of its four numbers
+    __half* p = quad == 0 ? kv4_by_quad(at, 256 * NG) : quad == 1 ? kv4_key_min(at, NG, g)
+              : kv4_by_quad(at, quad == 2 ? 576 * NG : 608 * NG);
+    *p = quad == 0 ? ks : quad == 1 ? km : quad == 2 ? vs : vm;
 }
 
-template <typename T>
+template <typename T, int NG>
 __global__ void __launch_bounds__(kKv4Threads)
 kv4_read_kernel(Kv4Cache c, T* k_out, T* v_out, const long long* slots, int tokens) {
     pdl_trigger();
     pdl_wait();
-    const int lanes = c.d == 128 ? 4 : 3;   // log2 of a row's
-    const long long row = ((long long)blockIdx.x * kKv4Threads + threadIdx.x) >> lanes;
-    const int l = threadIdx.x & ((1 << lanes) - 1), head = blockIdx.y;
+    const long long row = ((long long)blockIdx.x * kKv4Threads + threadIdx.x) / (4 * NG);
+    const int l = threadIdx.x % (4 * NG), g = l >> 2, quad = l & 3, head = blockIdx.y;
     if (row >= tokens) return;
     const long long slot = slots[row];
-    float x[8] = {};
+    float xk[8] = {}, xv[8] = {};
     if (slot >= c.n_pages * c.page) record_status(kStatusBadShape);
     if (slot >= 0 && slot < c.n_pages * c.page) {
-        const Kv4At at = kv4_at(c, slot, head, l >> 2, l & 3);
-        const uint32_t w = blockIdx.z == 0 ? *at.kc : (uint32_t)at.vc[0] | (uint32_t)at.vc[8 * (c.d / kKv4Group)] << 16;
-        const float s = __half2float(blockIdx.z == 0 ? *at.ks : *at.vs);
-        const float m = __half2float(blockIdx.z == 0 ? *at.km : *at.vm);
+        const Kv4At at = kv4_at(c, slot, head, NG, g);
+        const uint16_t* vc = kv4_value_code(at, NG, g, quad);
+        const uint32_t wk = *kv4_key_code(at, NG, g, quad), wv = vc[0] | (uint32_t)vc[8 * NG] << 16;
+        const float ks = __half2float(*kv4_by_quad(at, 256 * NG)), km = __half2float(*kv4_key_min(at, NG, g));
+        const float vs = __half2float(*kv4_by_quad(at, 576 * NG)), vm = __half2float(*kv4_by_quad(at, 608 * NG));
         #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = fmaf((float)((w >> (4 * e)) & 15u), s, m);
+        for (int e = 0; e < 8; ++e) {
+            xk[e] = fmaf(i2f_small((wk >> (4 * e)) & 15u), ks, km);
+            xv[e] = fmaf(i2f_small((wv >> (4 * e)) & 15u), vs, vm);
+        }
     }
-    store8((blockIdx.z ? v_out : k_out) + (row * c.n_kv + head) * c.d + 8 * l, x);
+    const long long at = (row * c.n_kv + head) * (32 * NG) + 8 * l;
+    store8(k_out + at, xk);
+    store8(v_out + at, xv);
 }
 
 cudaError_t kv4_append(const Kv4Cache& c, const HeadsIn& k, const HeadsIn& v, int type, const long long* slots,
@@ -453,8 +540,9 @@ cudaError_t kv4_append(const Kv4Cache& c, const HeadsIn& k, const HeadsIn& v, in
     const int vec = heads_aligned(k, type_size(type), n) && heads_aligned(v, type_size(type), n);
     const long long blocks = ((long long)tokens * (c.d / 8) + kKv4Threads - 1) / kKv4Threads;
     const cudaError_t e = by_type(type, [&](auto t) {
-        return launch_k(kv4_append_kernel<decltype(t)>, dim3((unsigned)blocks, c.n_kv, 2), dim3(kKv4Threads), 0, st, c,
-                        k, v, slots, tokens, vec);
+        using T = decltype(t);
+        return launch_k(c.d == 128 ? kv4_append_kernel<T, 4> : kv4_append_kernel<T, 2>, dim3((unsigned)blocks, c.n_kv),
+                        dim3(kKv4Threads), 0, st, c, k, v, slots, tokens, vec);
     });
     return e != cudaSuccess ? e : cudaGetLastError();
 }
@@ -465,8 +553,8 @@ cudaError_t kv4_read(const Kv4Cache& c, void* k_out, void* v_out, int type, cons
     const long long blocks = ((long long)tokens * (c.d / 8) + kKv4Threads - 1) / kKv4Threads;
     const cudaError_t e = by_type(type, [&](auto t) {
         using T = decltype(t);
-        return launch_k(kv4_read_kernel<T>, dim3((unsigned)blocks, c.n_kv, 2), dim3(kKv4Threads), 0, st, c,
-                        static_cast<T*>(k_out), static_cast<T*>(v_out), slots, tokens);
+        return launch_k(c.d == 128 ? kv4_read_kernel<T, 4> : kv4_read_kernel<T, 2>, dim3((unsigned)blocks, c.n_kv),
+                        dim3(kKv4Threads), 0, st, c, static_cast<T*>(k_out), static_cast<T*>(v_out), slots, tokens);
     });
     return e != cudaSuccess ? e : cudaGetLastError();
 }
