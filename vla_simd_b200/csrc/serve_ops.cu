@@ -163,13 +163,32 @@ qk_norm_rope_kernel(const __grid_constant__ RopeArgs a, int gs) {
     const bool on = lane < a.d / 8, turned = FULL || lane < a.rot / 8;
     const int c0 = turned ? 4 * lane : 8 * lane, c1 = turned ? a.rot / 2 + 4 * lane : 8 * lane + 4;
     constexpr int kRows = sizeof(TI) == 4 ? 3 : 4;
+    // the groups of a warp have the same pairs: each works out its share of the
+    // four (two groups: pairs e, e + 2; four and more: one each) and hands it on
     float2 co[2], si[2];
+    const int shared = min(n_sub, 4);
     #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        const float2 v = turned && on ? rope_turn(a.pos[(long long)axis[4 * lane + e] * a.tokens + t], turns[4 * lane + e])
-                                      : make_float2(1.f, 0.f);
-        (e & 1 ? co[e >> 1].y : co[e >> 1].x) = v.x;
-        (e & 1 ? si[e >> 1].y : si[e >> 1].x) = v.y;
+        float2 v = make_float2(1.f, 0.f);
+        if (e * shared < 4) {
+            const int pair = 4 * lane + e * shared + (sub & (shared - 1));
+            if (turned && on) v = rope_turn(a.pos[(long long)axis[pair] * a.tokens + t], turns[pair]);
+        }
+        if (e & 1) { co[e >> 1].y = v.x; si[e >> 1].y = v.y; }
+        else { co[e >> 1].x = v.x; si[e >> 1].x = v.y; }
+    }
+    if (shared == 2) {
+        const float2 c = co[0], s = si[0];   // pairs sub, sub + 2
+        co[0] = make_float2(__shfl_sync(0xffffffffu, c.x, lane), __shfl_sync(0xffffffffu, c.x, lane + gs));
+        co[1] = make_float2(__shfl_sync(0xffffffffu, c.y, lane), __shfl_sync(0xffffffffu, c.y, lane + gs));
+        si[0] = make_float2(__shfl_sync(0xffffffffu, s.x, lane), __shfl_sync(0xffffffffu, s.x, lane + gs));
+        si[1] = make_float2(__shfl_sync(0xffffffffu, s.y, lane), __shfl_sync(0xffffffffu, s.y, lane + gs));
+    } else if (shared == 4) {
+        const float c = co[0].x, s = si[0].x;   // pair sub & 3
+        co[0] = make_float2(__shfl_sync(0xffffffffu, c, lane), __shfl_sync(0xffffffffu, c, lane + gs));
+        co[1] = make_float2(__shfl_sync(0xffffffffu, c, lane + 2 * gs), __shfl_sync(0xffffffffu, c, lane + 3 * gs));
+        si[0] = make_float2(__shfl_sync(0xffffffffu, s, lane), __shfl_sync(0xffffffffu, s, lane + gs));
+        si[1] = make_float2(__shfl_sync(0xffffffffu, s, lane + 2 * gs), __shfl_sync(0xffffffffu, s, lane + 3 * gs));
     }
     const int step = a.per_token * n_sub;
     #pragma unroll 1
@@ -381,53 +400,56 @@ __device__ __forceinline__ __half* kv4_by_quad(const Kv4At& at, int byte) {
     return reinterpret_cast<__half*>(at.block + byte) + at.by_quad;
 }
 
-__device__ __forceinline__ float min_nan(float a, float b) {   // NaN if either is
+__device__ __forceinline__ float min_nan(float a, float b, float c) {   // NaN if one is
     float r;
-    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
-__device__ __forceinline__ float max_nan(float a, float b) {
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
     float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
 
 // codes of 8 channels (one nibble each) and the group's s, m; the group is
 // spread over the 4 lanes of a quad. The quotient (x - m) / s is first taken as
-// a product with 1 / (15 s), saturated to [0, 1]: good to 2^-20 of a step. Only
-// where that leaves the nearest code open (a step's middle within 2^-16: one
-// group in 500 of random values) is it divided.
+// one saturated fma with 1 / (15 s): good to 2^-17 + |m / s| 2^-21 of a step.
+// Only where that leaves the nearest code open (a step's middle is that near:
+// one group in 500 of random values) is it divided.
 __device__ __forceinline__ uint32_t kv4_quantize(const float (&x)[8], __half& s, __half& m) {
-    float lo = x[0], hi = x[0];
-    #pragma unroll
-    for (int i = 1; i < 8; ++i) {
-        lo = min_nan(lo, x[i]);
-        hi = max_nan(hi, x[i]);
+    float lo = min_nan(min_nan(x[0], x[1], x[2]), min_nan(x[3], x[4], x[5]), min_nan(x[6], x[7], x[7]));
+    float hi = max_nan(max_nan(x[0], x[1], x[2]), max_nan(x[3], x[4], x[5]), max_nan(x[6], x[7], x[7]));
+    {
+        const float a = __shfl_xor_sync(0xffffffffu, lo, 1), b = __shfl_xor_sync(0xffffffffu, lo, 2);
+        const float c = __shfl_xor_sync(0xffffffffu, lo, 3);
+        lo = min_nan(lo, a, min_nan(b, c, c));
+        const float d = __shfl_xor_sync(0xffffffffu, hi, 1), e = __shfl_xor_sync(0xffffffffu, hi, 2);
+        const float f = __shfl_xor_sync(0xffffffffu, hi, 3);
+        hi = max_nan(hi, d, max_nan(e, f, f));
     }
-    #pragma unroll
-    for (int o = 1; o < 4; o <<= 1) {
-        lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-        hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-    }
-    const bool bad = !(fmaxf(fabsf(lo), fabsf(hi)) <= 3.402823466e38f) || lo != lo;
+    const bool bad = !(fabsf(lo) <= 3.402823466e38f && fabsf(hi) <= 3.402823466e38f);
     lo = fminf(fmaxf(lo, -65504.0f), 65504.0f);
     hi = fminf(fmaxf(hi, -65504.0f), 65504.0f);
     s = __float2half_rn(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f));
     m = __float2half_rn(lo);
     if (bad) s = m = __ushort_as_half(0x7fff);
     const float sf = __half2float(s), mf = __half2float(m);
-    const float inv = sf > 0.0f ? __fdividef(1.0f, 15.0f * sf) : 0.0f;
+    const float inv = sf > 0.0f ? __fdividef(1.0f, 15.0f * sf) : 0.0f, off = -mf * inv;
     // the code in the low bits of 1.5 * 2^23 + code
     uint32_t w = 0;
     float nearest = 0.f;   // the largest distance of a quotient from its code
     #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float f = __saturatef(__fsub_rn(x[i], mf) * inv);
-        const float u = fmaf(f, 15.0f, kRoundConst);
-        nearest = fmaxf(nearest, fabsf(fmaf(f, 15.0f, kRoundConst - u)));
-        w += (__float_as_uint(u) - 0x4B400000u) << (4 * i);
+    for (int i = 0; i < 8; i += 2) {
+        const float2 f = make_float2(__saturatef(fmaf(x[i], inv, off)), __saturatef(fmaf(x[i + 1], inv, off)));
+        const float2 k15 = make_float2(15.f, 15.f), kr = make_float2(kRoundConst, kRoundConst);
+        const float2 u = fma2(f, k15, kr);
+        const float2 d = fma2(f, k15, fma2(u, make_float2(-1.f, -1.f), kr));
+        nearest = fmaxf(nearest, fmaxf(fabsf(d.x), fabsf(d.y)));
+        w += __float_as_uint(u.x) << (4 * i);
+        w += __float_as_uint(u.y) << (4 * i + 4);
     }
-    if (nearest > 0.5f - 1.0f / 65536.0f) {
+    w -= 0x3F400000u;   // what the eight shifted 0x4B400000 (1.5 * 2^23) add up to
+    if (!(nearest <= 0.5f - 1.0f / 65536.0f - fabsf(off) * (15.0f / 2097152.0f))) {
         w = 0;
         #pragma unroll 1
         for (int i = 0; i < 8; ++i) {
@@ -459,15 +481,28 @@ __device__ __forceinline__ void load8(const T* p, bool vec, float (&x)[8]) {
     }
 }
 
+// 8 channels of each lane to p + 8 * lane (whole warp). fp32: neighbouring lanes
+// trade halves first, so that each store of the warp is one run of bytes.
 template <typename T>
-__device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
-    constexpr int N = sizeof(T) == 4 ? 4 : 8;
-    #pragma unroll
-    for (int h = 0; h < 8 / N; ++h) {
-        Pack<T, N> v;
+__device__ __forceinline__ void store8(T* p, float (&x)[8], bool on) {
+    if constexpr (sizeof(T) == 4) {
+        const bool odd = threadIdx.x & 1;
         #pragma unroll
-        for (int i = 0; i < N; ++i) v.v[i] = from_f<T>(x[h * N + i]);
-        *reinterpret_cast<Pack<T, N>*>(p + h * N) = v;
+        for (int i = 0; i < 4; ++i) {
+            const float y = __shfl_xor_sync(0xffffffffu, odd ? x[i] : x[i + 4], 1);
+            if (odd) x[i] = y;
+            else x[i + 4] = y;
+        }
+        // even: its 0..3 and the odd lane's 0..3; odd: the even lane's 4..7 and its 4..7
+        if (on) {
+            *reinterpret_cast<float4*>(p + (odd ? -4 : 0)) = make_float4(x[0], x[1], x[2], x[3]);
+            *reinterpret_cast<float4*>(p + (odd ? 4 : 8)) = make_float4(x[4], x[5], x[6], x[7]);
+        }
+    } else if (on) {
+        Pack<T, 8> v;
+        #pragma unroll
+        for (int i = 0; i < 8; ++i) v.v[i] = from_f<T>(x[i]);
+        *reinterpret_cast<Pack<T, 8>*>(p) = v;
     }
 }
 
@@ -512,8 +547,8 @@ kv4_read_kernel(Kv4Cache c, T* k_out, T* v_out, const long long* slots, int toke
     pdl_wait();
     const long long row = ((long long)blockIdx.x * kKv4Threads + threadIdx.x) / (4 * NG);
     const int l = threadIdx.x % (4 * NG), g = l >> 2, quad = l & 3, head = blockIdx.y;
-    if (row >= tokens) return;
-    const long long slot = slots[row];
+    const bool on = row < tokens;
+    const long long slot = on ? slots[row] : -1;
     float xk[8] = {}, xv[8] = {};
     if (slot >= c.n_pages * c.page) record_status(kStatusBadShape);
     if (slot >= 0 && slot < c.n_pages * c.page) {
@@ -529,8 +564,8 @@ kv4_read_kernel(Kv4Cache c, T* k_out, T* v_out, const long long* slots, int toke
         }
     }
     const long long at = (row * c.n_kv + head) * (32 * NG) + 8 * l;
-    store8(k_out + at, xk);
-    store8(v_out + at, xv);
+    store8(k_out + at, xk, on);
+    store8(v_out + at, xv, on);
 }
 
 cudaError_t kv4_append(const Kv4Cache& c, const HeadsIn& k, const HeadsIn& v, int type, const long long* slots,
