@@ -10,6 +10,7 @@
 
 #include <algorithm>
 #include <climits>
+#include <cstdlib>
 
 namespace vsb {
 
@@ -140,19 +141,21 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
 // / 8) have a row; lane l the two quads of channels [c0, c0 + 4) and [c1, c1 + 4)
 // that pair up with each other, so a row is rotated without exchanging values and
 // a lane's four sines and cosines, times the norm's weights, serve every head
-// from registers: inv * (x0 (w0 cos) - x1 (w1 sin)). Two channels an instruction
-// (f32x2): at one instruction a channel the kernel was bound by issue (190 a row,
-// 32 us at 4099 tokens of 40 heads of 128). kRows rows a lane are loaded before
-// the first is used.
-template <typename TI, typename TO, bool FULL>   // FULL: every channel turns
+// from registers: inv * (x0 (w0 cos) - x1 (w1 sin)), two channels an instruction
+// (f32x2). What bounds it besides HBM is issue: 190 instructions a row at one
+// channel an instruction (32 us at 4099 tokens of 40 heads of 128), hence D, the
+// usual widths with every channel turned, known to the compiler (0: any). kRows
+// rows a lane are loaded before the first is used.
+template <typename TI, typename TO, int D>
 __global__ void __launch_bounds__(kRopeThreads, 4)
-qk_norm_rope_kernel(const __grid_constant__ RopeArgs a, int gs) {
+qk_norm_rope_kernel(const __grid_constant__ RopeArgs a, int gs_any) {
     __shared__ double turns[kMaxPairs];
     __shared__ unsigned char axis[kMaxPairs];
+    const int gs = D ? D / 8 : gs_any, d = D ? D : a.d, rot = D ? D : a.rot;
     const int wid = blockIdx.x * (kRopeThreads / 32) + (threadIdx.x >> 5);
     const int t = wid / a.per_token, share = wid - t * a.per_token;
     const int lane = threadIdx.x & (gs - 1), sub = (threadIdx.x & 31) / gs, n_sub = 32 / gs;
-    for (int i = threadIdx.x; i < a.rot / 2; i += kRopeThreads) {   // once a CTA: lanes index it apart
+    for (int i = threadIdx.x; i < rot / 2; i += kRopeThreads) {   // once a CTA: lanes index it apart
         turns[i] = a.tab.turns[i];
         axis[i] = a.tab.axis[i];
     }
@@ -160,11 +163,11 @@ qk_norm_rope_kernel(const __grid_constant__ RopeArgs a, int gs) {
     pdl_trigger();
     pdl_wait();
     if (t >= a.tokens) return;
-    const bool on = lane < a.d / 8, turned = FULL || lane < a.rot / 8;
-    const int c0 = turned ? 4 * lane : 8 * lane, c1 = turned ? a.rot / 2 + 4 * lane : 8 * lane + 4;
+    const bool on = D || lane < d / 8, turned = D || lane < rot / 8;
+    const int c0 = turned ? 4 * lane : 8 * lane, c1 = D ? c0 + D / 2 : turned ? rot / 2 + 4 * lane : 8 * lane + 4;
     constexpr int kRows = sizeof(TI) == 4 ? 3 : 4;
     // the groups of a warp have the same pairs: each works out its share of the
-    // four (two groups: pairs e, e + 2; four and more: one each) and hands it on
+    // four (two groups: pairs sub, sub + 2; four and more: one each) and hands it on
     float2 co[2], si[2];
     const int shared = min(n_sub, 4);
     #pragma unroll
@@ -178,13 +181,13 @@ qk_norm_rope_kernel(const __grid_constant__ RopeArgs a, int gs) {
         else { co[e >> 1].x = v.x; si[e >> 1].x = v.y; }
     }
     if (shared == 2) {
-        const float2 c = co[0], s = si[0];   // pairs sub, sub + 2
+        const float2 c = co[0], s = si[0];
         co[0] = make_float2(__shfl_sync(0xffffffffu, c.x, lane), __shfl_sync(0xffffffffu, c.x, lane + gs));
         co[1] = make_float2(__shfl_sync(0xffffffffu, c.y, lane), __shfl_sync(0xffffffffu, c.y, lane + gs));
         si[0] = make_float2(__shfl_sync(0xffffffffu, s.x, lane), __shfl_sync(0xffffffffu, s.x, lane + gs));
         si[1] = make_float2(__shfl_sync(0xffffffffu, s.y, lane), __shfl_sync(0xffffffffu, s.y, lane + gs));
     } else if (shared == 4) {
-        const float c = co[0].x, s = si[0].x;   // pair sub & 3
+        const float c = co[0].x, s = si[0].x;
         co[0] = make_float2(__shfl_sync(0xffffffffu, c, lane), __shfl_sync(0xffffffffu, c, lane + gs));
         co[1] = make_float2(__shfl_sync(0xffffffffu, c, lane + 2 * gs), __shfl_sync(0xffffffffu, c, lane + 3 * gs));
         si[0] = make_float2(__shfl_sync(0xffffffffu, s, lane), __shfl_sync(0xffffffffu, s, lane + gs));
@@ -194,12 +197,11 @@ qk_norm_rope_kernel(const __grid_constant__ RopeArgs a, int gs) {
     #pragma unroll 1
     for (int part = 0; part < 2; ++part) {
         const int nh = part ? a.n_kv : a.n_q;
+        if (nh == 0) continue;
         const HeadsIn& in = part ? a.k : a.q;
-        const int first = share * n_sub + sub;
-        const TI* src = static_cast<const TI*>(in.p) + (long long)t * in.tok + (long long)first * in.head;
-        TO* dst = static_cast<TO*>(part ? a.k_out : a.q_out) + ((long long)t * nh + first) * a.d;
-        const long long src_step = step * in.head;
-        const int dst_step = step * a.d;
+        const TI* src = static_cast<const TI*>(in.p) + (long long)t * in.tok + c0;
+        TO* dst = static_cast<TO*>(part ? a.k_out : a.q_out) + (long long)t * nh * d + c0;
+        const int head = (int)in.head;
         const float* wp = part ? a.kw : a.qw;
         float2 w0[2], w1[2];
         w0[0] = w0[1] = w1[0] = w1[1] = make_float2(1.f, 1.f);
@@ -207,7 +209,7 @@ qk_norm_rope_kernel(const __grid_constant__ RopeArgs a, int gs) {
             load_quad(wp + c0, w0);
             load_quad(wp + c1, w1);
         }
-        // x0 -> x0 * f00 - x1 * f01, x1 -> x1 * f11 + x0 * f10
+        // x0 -> x0 * f00 + x1 * f01, x1 -> x1 * f11 + x0 * f10
         float2 f00[2], f01[2], f10[2], f11[2];
         #pragma unroll
         for (int e = 0; e < 2; ++e) {
@@ -216,32 +218,34 @@ qk_norm_rope_kernel(const __grid_constant__ RopeArgs a, int gs) {
             f10[e] = mul2(w0[e], si[e]);
             f11[e] = mul2(w1[e], co[e]);
         }
-        for (int h0 = first; h0 - sub < nh; h0 += kRows * step) {
+        for (int h0 = share * n_sub; h0 < nh; h0 += kRows * step) {
             Quad<TI> x[kRows][2];
             #pragma unroll
-            for (int u = 0; u < kRows; ++u) {
-                x[u][0] = x[u][1] = Quad<TI>{};
-                if (h0 + u * step < nh && on) {
-                    x[u][0] = *reinterpret_cast<const Quad<TI>*>(src + c0);
-                    x[u][1] = *reinterpret_cast<const Quad<TI>*>(src + c1);
+            for (int u = 0; u < kRows; ++u) {   // past the last head: the last one again
+                const TI* p = src + (long long)min(h0 + sub + u * step, nh - 1) * head;
+                if (D || on) {
+                    x[u][0] = *reinterpret_cast<const Quad<TI>*>(p);
+                    x[u][1] = *reinterpret_cast<const Quad<TI>*>(p + (c1 - c0));
+                } else {
+                    x[u][0] = x[u][1] = Quad<TI>{};
                 }
-                src += src_step;
             }
             #pragma unroll
             for (int u = 0; u < kRows; ++u) {
-                if (h0 - sub + u * step >= nh) break;   // the same for the whole warp
                 const float2 y0[2] = {x[u][0].lo(), x[u][0].hi()}, y1[2] = {x[u][1].lo(), x[u][1].hi()};
                 float2 inv2 = make_float2(1.f, 1.f);
                 if (wp) {
                     const float2 s2 = fma2(y0[0], y0[0], fma2(y0[1], y0[1], fma2(y1[0], y1[0], mul2(y1[1], y1[1]))));
                     float ss = s2.x + s2.y;
-                    for (int o = gs >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+                    #pragma unroll
+                    for (int o = 16; o > 0; o >>= 1)
+                        if (o < gs) ss += __shfl_xor_sync(0xffffffffu, ss, o);
                     inv2.x = inv2.y = rsqrtf(fmaf(ss, a.inv_d, a.eps));
                 }
                 float2 r0[2], r1[2];
                 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    if (FULL || turned) {
+                    if (turned) {
                         r0[e] = mul2(fma2(y0[e], f00[e], mul2(y1[e], f01[e])), inv2);
                         r1[e] = mul2(fma2(y1[e], f11[e], mul2(y0[e], f10[e])), inv2);
                     } else {
@@ -249,11 +253,11 @@ qk_norm_rope_kernel(const __grid_constant__ RopeArgs a, int gs) {
                         r1[e] = mul2(mul2(y1[e], w1[e]), inv2);
                     }
                 }
-                if (h0 + u * step < nh && on) {
-                    *reinterpret_cast<Quad<TO>*>(dst + c0) = Quad<TO>::of(r0[0], r0[1]);
-                    *reinterpret_cast<Quad<TO>*>(dst + c1) = Quad<TO>::of(r1[0], r1[1]);
+                if (h0 + sub + u * step < nh && on) {
+                    TO* p = dst + (h0 + sub + u * step) * d;
+                    *reinterpret_cast<Quad<TO>*>(p) = Quad<TO>::of(r0[0], r0[1]);
+                    *reinterpret_cast<Quad<TO>*>(p + (c1 - c0)) = Quad<TO>::of(r1[0], r1[1]);
                 }
-                dst += dst_step;
             }
         }
     }
@@ -321,7 +325,8 @@ cudaError_t qk_norm_rope(void* q_out, void* k_out, int out_type, const HeadsIn& 
     RopeArgs a{q, k, q_out, k_out, pos, qw, kw, eps, 1.0f / (float)d, tokens, n_q, n_kv, d, rot, 1, tab};
     const size_t os = type_size(out_type);
     const bool quads = d % 8 == 0 && rot % 8 == 0 && heads_aligned(q, type_size(in_type), 4) &&
-                       (n_kv == 0 || heads_aligned(k, type_size(in_type), 4)) &&
+                       (n_kv == 0 || heads_aligned(k, type_size(in_type), 4)) && std::abs(q.head) < INT_MAX &&
+                       (n_kv == 0 || std::abs(k.head) < INT_MAX) &&
                        (reinterpret_cast<uintptr_t>(q_out) | reinterpret_cast<uintptr_t>(k_out)) % (4 * os) == 0 &&
                        (reinterpret_cast<uintptr_t>(qw) | reinterpret_cast<uintptr_t>(kw)) % 16 == 0;
     int gs = 1;
@@ -340,8 +345,10 @@ cudaError_t qk_norm_rope(void* q_out, void* k_out, int out_type, const HeadsIn& 
                 return launch_k(qk_norm_rope_any_kernel<TI, TO>, dim3(tokens), dim3(kRopeThreads),
                                 sizeof(float2) * (rot / 2), st, a);
             const dim3 grid((unsigned)((warps + 7) / 8));
-            return rot == d ? launch_k(qk_norm_rope_kernel<TI, TO, true>, grid, dim3(kRopeThreads), 0, st, a, gs)
-                            : launch_k(qk_norm_rope_kernel<TI, TO, false>, grid, dim3(kRopeThreads), 0, st, a, gs);
+            const auto kernel = rot == d && d == 128 ? qk_norm_rope_kernel<TI, TO, 128>
+                              : rot == d && d == 64  ? qk_norm_rope_kernel<TI, TO, 64>
+                                                     : qk_norm_rope_kernel<TI, TO, 0>;
+            return launch_k(kernel, grid, dim3(kRopeThreads), 0, st, a, gs);
         });
     });
     return e != cudaSuccess ? e : cudaGetLastError();
