@@ -422,7 +422,7 @@ __device__ __forceinline__ float max_nan(float a, float b, float c) {
 // spread over the 4 lanes of a quad. The quotient (x - m) / s is first taken as
 // one saturated fma with 1 / (15 s): good to 2^-17 + |m / s| 2^-21 of a step.
 // Only where that leaves the nearest code open (a step's middle is that near:
-// one group in 500 of random values) is it divided.
+// one bf16 value in 1200, one lane in 170) is it divided.
 __device__ __forceinline__ uint32_t kv4_quantize(const float (&x)[8], __half& s, __half& m) {
     float lo = min_nan(min_nan(x[0], x[1], x[2]), min_nan(x[3], x[4], x[5]), min_nan(x[6], x[7], x[7]));
     float hi = max_nan(max_nan(x[0], x[1], x[2]), max_nan(x[3], x[4], x[5]), max_nan(x[6], x[7], x[7]));
@@ -456,15 +456,23 @@ __device__ __forceinline__ uint32_t kv4_quantize(const float (&x)[8], __half& s,
         w += __float_as_uint(u.y) << (4 * i + 4);
     }
     w -= 0x3F400000u;   // what the eight shifted 0x4B400000 (1.5 * 2^23) add up to
-    if (!(nearest <= 0.5f - 1.0f / 65536.0f - fabsf(off) * (15.0f / 2097152.0f))) {
-        w = 0;
-        #pragma unroll 1
+    const float open = 0.5f - 1.0f / 65536.0f - fabsf(off) * (15.0f / 2097152.0f);
+    if (!(nearest <= open)) {   // NaN, too: its codes are 0 either way
+        uint32_t which = 0;
+        #pragma unroll
         for (int i = 0; i < 8; ++i) {
+            const float f = __saturatef(fmaf(x[i], inv, off));
+            const float d = fmaf(f, 15.0f, kRoundConst - fmaf(f, 15.0f, kRoundConst));
+            which |= fabsf(d) > open ? 1u << i : 0u;
+        }
+        while (which) {
+            const int i = __ffs(which) - 1;
+            which &= which - 1;
             float xi = x[0];
             #pragma unroll
             for (int y = 1; y < 8; ++y) xi = i == y ? x[y] : xi;
-            const float c = sf > 0.0f ? rintf(__fdiv_rn(__fsub_rn(xi, mf), sf)) : 0.0f;
-            w |= (uint32_t)(int)fminf(fmaxf(c, 0.0f), 15.0f) << (4 * i);
+            const float c = fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(xi, mf), sf)), 0.0f), 15.0f);
+            w = (w & ~(15u << (4 * i))) | (uint32_t)(int)c << (4 * i);
         }
     }
     return w;
