@@ -447,7 +447,8 @@ kv4_attention_kernel(const __grid_constant__ Kv4AttDev p) {
             }
             #pragma unroll
             for (int g = 0; g < NG; ++g) {
-                uint32_t b0, b1, c0 = 0u, c1 = 0u;   // p * s of row n (and what it leaves)
+                uint32_t b0, b1;                          // p * s of row n
+                [[maybe_unused]] uint32_t c0 = 0u, c1 = 0u;   // and what it leaves
                 if constexpr (kSplit) {
                     const float2 s0 = unpack_h2(vs[2 * g]), s1 = unpack_h2(vs[2 * g + 1]);
                     split_h2(pw[0].x * s0.x, pw[0].y * s0.y, b0, c0);

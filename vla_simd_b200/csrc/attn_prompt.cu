@@ -11,9 +11,11 @@
 // the group) pairs, token-major: the keys of a group are loaded once for all of
 // its heads, and a causal tile spans 128 / group tokens, which keeps what the
 // mask throws away small. Warps: 0-3 and 4-7 the softmax of tile 0 and 1 (thread
-// = row = TMEM lane), 8 issues the matrix products, 9 the TMA loads of a ring of
-// K and V tiles. While one tile's softmax runs, the tensor core has the other's
-// products.
+// = row = TMEM lane), 8 and 9 issue the matrix products of tile 0 and 1 (each
+// waits for its own tile alone: with one warp for both, the tiles ran in
+// lockstep, 4130 cycles a pair of blocks), 10 the TMA loads of a ring of K and V
+// tiles, 11 looks over the value tiles that are not seen in full. While one
+// tile's softmax runs, the tensor core has the other's products.
 //
 // m only follows the true maximum when it is more than 2^8 behind (P then stays
 // below 2^8, far inside bf16 and fp16): O is rescaled in TMEM that rarely, by
@@ -151,6 +153,51 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     return d;
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
+// The registers of a tcgen05.ld are there once tmem_ld_wait() has returned: no
+// use of them may be moved in front of it.
+template <int N>
+__device__ __forceinline__ void tmem_ready(uint32_t (&r)[N]) {
+    #pragma unroll
+    for (int i = 0; i < N; ++i) asm volatile("" : "+r"(r[i]));
+}
+
+// 2^x for x in [-126, 127] on the FMA pipe: x = n + f, |f| <= 1/2, 2^f by the
+// polynomial of least relative error (fitted to 2^f by Remez exchange: 2^-13.7 at
+// degree 3, 2^-18.5 at degree 4), n added to the exponent. Below -126 it stays at
+// 2^-126, which the weights' type rounds to nothing beside a row's largest.
+template <bool FINE>
+__device__ __forceinline__ float2 ex2_poly(float2 x) {
+    x.x = fmaxf(x.x, -126.f);
+    x.y = fmaxf(x.y, -126.f);
+    const float2 big = make_float2(kRoundConst, kRoundConst), nbig = make_float2(-kRoundConst, -kRoundConst);
+    const float2 t = add2(x, big);
+    const float2 f = fma2(add2(t, nbig), make_float2(-1.f, -1.f), x);
+    float2 p;
+    if constexpr (FINE) {
+        p = fma2(make_float2(0.00957010210f, 0.00957010210f), f, make_float2(0.0559178628f, 0.0559178628f));
+        p = fma2(p, f, make_float2(0.240247443f, 0.240247443f));
+        p = fma2(p, f, make_float2(0.693121791f, 0.693121791f));
+        p = fma2(p, f, make_float2(0.999999285f, 0.999999285f));
+    } else {
+        p = fma2(make_float2(0.0551716685f, 0.0551716685f), f, make_float2(0.242611125f, 0.242611125f));
+        p = fma2(p, f, make_float2(0.693260968f, 0.693260968f));
+        p = fma2(p, f, make_float2(0.999928057f, 0.999928057f));
+    }
+    p.x = __int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23));
+    p.y = __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23));
+    return p;
+}
+
+#ifndef PA_POLY
+#define PA_POLY 0
+#endif
+
 // What a CTA works on: tile t has rows of queries [tok[t], tok[t] + n_tok[t])
 // of the sequence and sees the first keys[t] of its lk keys.
 struct PromptJob {
@@ -162,7 +209,7 @@ __global__ void __launch_bounds__(kPaThreads, 1)
 prompt_tc_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__ CUtensorMap mq,
                  const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv) {
     constexpr bool kBf16 = sizeof(T) == 2 && !std::is_same<T, __half>::value;
-    constexpr int kStages = pa_stages(D), kCB = D / 64;
+    constexpr int kStages = pa_stages(D), kCB = D / 64, kPoly = PA_POLY;
     constexpr uint32_t kTile = kCB * kPaBoxBytes;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* sm = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -171,9 +218,11 @@ prompt_tc_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__ C
     uint64_t* q_full = reinterpret_cast<uint64_t*>(ring + kStages * kTile);
     uint64_t* kv_full = q_full + 1;
     uint64_t* kv_empty = kv_full + kStages;
-    uint64_t* s_full = kv_empty + kStages;
+    uint64_t* v_raw = kv_empty + kStages;   // value tiles that warp 11 looks over first
+    uint64_t* s_full = v_raw + kStages;
     uint64_t* p_full = s_full + 2;
-    uint64_t* o_done = p_full + 2;
+    uint64_t* turn = p_full + 2;
+    uint64_t* o_done = turn + 2;
     uint32_t* tslot = reinterpret_cast<uint32_t*>(o_done + 2);
     PromptJob* job = reinterpret_cast<PromptJob*>(tslot + 2);
 
@@ -185,11 +234,13 @@ prompt_tc_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__ C
         mbar_init(q_full, 1);
         for (int i = 0; i < kStages; ++i) {
             mbar_init(kv_full + i, 1);
-            mbar_init(kv_empty + i, 1);
+            mbar_init(kv_empty + i, 2);
+            mbar_init(v_raw + i, 1);
         }
         for (int t = 0; t < 2; ++t) {
             mbar_init(s_full + t, 1);
             mbar_init(p_full + t, 128);
+            mbar_init(turn + t, 1);
             mbar_init(o_done + t, 1);
         }
         fence_mbar_init();
@@ -252,7 +303,12 @@ prompt_tc_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__ C
 
     if (warp >= 8) {
         regs_dec<kPaRegsRest>();
-        if (warp == 9 && nblk > 0) {
+        // the fewest keys any row here sees: past them some weights are masked to 0
+        const int clear_all = nblk > 0 ? prompt_limit(a, seq, job->n_tok[0] > 0 ? job->tok[0] : job->tok[1], job->lq, job->lk) : 0;
+        const int masked0 = clear_all / kPaKeys;   // the first block that is not seen in full
+        // masked value blocks go round the ring's stages with this period
+        constexpr int kPeriod = kStages % 2 ? kStages : kStages / 2;
+        if (warp == 10 && nblk > 0) {
             // ---- loads: Q tiles, then K and V of each block through the ring
             if (lane == 0) {
                 mbar_arrive_expect_tx(q_full, (uint32_t)((nblk0 > 0) + (nblk1 > 0)) * kCB * 128u * (uint32_t)(a.gp * a.tile_tok));
@@ -264,96 +320,114 @@ prompt_tc_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__ C
                 for (; i < 2 * nblk; ++i) {
                     const int st = i % kStages;
                     if (i >= kStages && !mbar_wait(kv_empty + st, (uint32_t)(i / kStages - 1) & 1u)) break;
-                    mbar_arrive_expect_tx(kv_full + st, kTile);
+                    uint64_t* bar = (i & 1) && (i >> 1) >= masked0 ? v_raw + st : kv_full + st;
+                    mbar_arrive_expect_tx(bar, kTile);
                     for (int c = 0; c < kCB; ++c)
-                        tma_load_3d(ring + st * kTile + c * kPaBoxBytes, (i & 1) ? &mv : &mk, kv_full + st, 64 * c, kvh,
+                        tma_load_3d(ring + st * kTile + c * kPaBoxBytes, (i & 1) ? &mv : &mk, bar, 64 * c, kvh,
                                     job->k0 + (i >> 1) * kPaKeys);
                 }
                 // every copy has landed before the CTA may leave (after a wait that gave up, too)
                 const uint64_t until = globaltimer_ns() + kWaitLimitNs;
                 mbar_wait_until(q_full, 0, until);
-                for (int x = max(0, i - kStages); x < i; ++x)
-                    mbar_wait_until(kv_full + x % kStages, (uint32_t)(x / kStages) & 1u, until);
+                for (int x = max(0, i - kStages); x < i; ++x) {
+                    if ((x & 1) && (x >> 1) >= masked0)
+                        mbar_wait_until(v_raw + x % kStages, (uint32_t)(((x >> 1) - masked0) / kPeriod) & 1u, until);
+                    else
+                        mbar_wait_until(kv_full + x % kStages, (uint32_t)(x / kStages) & 1u, until);
+                }
             }
-        } else if (warp == 8 && nblk > 0) {
-            // ---- matrix products
+        } else if (warp == 11) {
+            // ---- value blocks that some row does not see all of: 0 * v has to be 0. Rows past the
+            // sequence become zeros; a NaN or an infinity in front of its end is left to the rows that
+            // see it, and the others are done again one by one.
+            for (int j = masked0; j < nblk; ++j) {
+                const int st = (2 * j + 1) % kStages;
+                if (!__all_sync(0xffffffffu, mbar_wait(v_raw + st, (uint32_t)((j - masked0) / kPeriod) & 1u))) break;
+                uint8_t* vt = ring + st * kTile;
+                const int valid = min(job->lk - j * kPaKeys, kPaKeys);
+                constexpr uint32_t kExp = kBf16 ? 0x7F80u : 0x7C00u;
+                bool bad = false;
+                for (int c = 0; c < kCB; ++c)
+                    #pragma unroll 8
+                    for (int x = lane; x < (int)kPaBoxBytes / 16; x += 32) {
+                        uint4* p = reinterpret_cast<uint4*>(vt + c * kPaBoxBytes) + x;
+                        if (x >= valid * 8) {
+                            *p = make_uint4(0u, 0u, 0u, 0u);
+                        } else {
+                            const uint4 w = *p;
+                            const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+                            #pragma unroll
+                            for (int y = 0; y < 4; ++y)
+                                bad |= (ws[y] & kExp) == kExp || (ws[y] >> 16 & kExp) == kExp;
+                        }
+                    }
+                if (bad) job->bad = 1;
+                __threadfence_block();
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(kv_full + st);
+            }
+        } else if (warp < 10 && nblk > 0) {
+            // ---- matrix products of tile t; a ring stage is free when both warps are past it
+            const int t = warp - 8, nb = t ? nblk1 : nblk0;
             constexpr uint32_t kPV = idesc_f16(kBf16, D, true, false);
             const uint32_t kQK = a.negate ? idesc_f16(kBf16, kPaKeys, false, true) : idesc_f16(kBf16, kPaKeys, false, false);
-            // the fewest keys any row here sees: past them some weights are masked to 0
-            const int first_tok = job->n_tok[0] > 0 ? job->tok[0] : job->tok[1];
-            const int clear = prompt_limit(a, seq, first_tok, job->lq, job->lk);
+            const uint64_t dq = sw128_kmajor_desc(smem_u32(sq + t * kTile)), dk = sw128_kmajor_desc(smem_u32(ring));
+            const uint64_t dv = sw128_mnmajor_desc(smem_u32(ring));
+            const uint32_t tS = tmem + 128 * t, tO = tmem + 256 + 128 * t;
             auto wait = [](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)) != 0; };
             bool ok = wait(q_full, 0);
-            auto qk = [&](int t, int j) {
-                const int i = 2 * j, st = i % kStages;
-                ok = ok && wait(kv_full + st, (uint32_t)(i / kStages) & 1u);
-                if (!ok) return;
-                tc_fence_after();
-                if (lane == 0) {
-                    const uint32_t qa = smem_u32(sq + t * kTile), kb = smem_u32(ring + st * kTile);
-                    #pragma unroll
-                    for (int k = 0; k < D / 16; ++k)
-                        umma_f16_ss(tmem + 128 * t, sw128_kmajor_desc(qa + (k >> 2) * kPaBoxBytes + (k & 3) * 32),
-                                    sw128_kmajor_desc(kb + (k >> 2) * kPaBoxBytes + (k & 3) * 32), kQK, k > 0);
-                    umma_commit(s_full + t);
+            auto k_there = [&](int j) { return wait(kv_full + 2 * j % kStages, (uint32_t)(2 * j / kStages) & 1u); };
+            auto qk = [&](int j) {   // one thread
+                const int st = 2 * j % kStages;
+                const uint64_t dks = dk + st * (kTile >> 4);
+                #pragma unroll
+                for (int k = 0; k < D / 16; ++k) {   // 32 bytes a step, 64 channels a box
+                    const int off = ((k >> 2) * kPaBoxBytes + (k & 3) * 32) >> 4;
+                    umma_f16_ss(tS, dq + off, dks + off, kQK, k > 0);
                 }
+                umma_commit(s_full + t);
+                umma_commit(kv_empty + st);
+            };
+            // a tile without block i / 2 passes it on, once it is there (one arrival a round)
+            auto pass = [&](int i) {
+                ok = ok && wait(kv_full + i % kStages, (uint32_t)(i / kStages) & 1u);
+                if (ok && lane == 0) mbar_arrive(kv_empty + i % kStages);
                 __syncwarp();
             };
-            if (nblk0 > 0) qk(0, 0);
-            if (nblk1 > 0) qk(1, 0);
-            if (lane == 0 && ok) umma_commit(kv_empty + 0);
-            int scrubbed = -1;
+            if (nb > 0) {
+                ok = ok && k_there(0);
+                tc_fence_after();
+                if (ok && lane == 0) qk(0);
+                __syncwarp();
+            } else {
+                pass(0);
+            }
+            const int nb_other = t ? nblk0 : nblk1;
             for (int j = 0; j < nblk && ok; ++j) {
                 const int iv = 2 * j + 1, sv = iv % kStages;
-                for (int t = 0; t < 2 && ok; ++t) {
-                    const int nb = t ? nblk1 : nblk0;
-                    if (j < nb) {
-                        ok = wait(kv_full + sv, (uint32_t)(iv / kStages) & 1u);
-                        if (ok && scrubbed < j && (j + 1) * kPaKeys > clear) {
-                            // a block that some row does not see all of: 0 * v has to be 0. Rows past the
-                            // sequence become zeros; a NaN or an infinity in front of its end is left to
-                            // the rows that see it, and the others are done again one by one.
-                            scrubbed = j;
-                            uint8_t* vt = ring + sv * kTile;
-                            const int valid = min(job->lk - j * kPaKeys, kPaKeys);
-                            constexpr uint32_t kExp = kBf16 ? 0x7F80u : 0x7C00u;
-                            bool bad = false;
-                            for (int c = 0; c < kCB; ++c)
-                                for (int x = lane; x < (int)kPaBoxBytes / 16; x += 32) {
-                                    uint4* p = reinterpret_cast<uint4*>(vt + c * kPaBoxBytes) + x;
-                                    if (x >= valid * 8) {
-                                        *p = make_uint4(0u, 0u, 0u, 0u);
-                                    } else {
-                                        const uint4 w = *p;
-                                        const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
-                                        #pragma unroll
-                                        for (int y = 0; y < 4; ++y)
-                                            bad |= (ws[y] & kExp) == kExp || (ws[y] >> 16 & kExp) == kExp;
-                                    }
-                                }
-                            if (bad) job->bad = 1;
-                            __threadfence_block();
-                            fence_proxy_async_smem();
-                            __syncwarp();
-                        }
-                        ok = ok && wait(p_full + t, (uint32_t)j & 1u);
-                        if (!ok) break;
-                        tc_fence_after();
-                        if (lane == 0) {
-                            const uint32_t va = smem_u32(ring + sv * kTile);
-                            #pragma unroll
-                            for (int k = 0; k < kPaKeys / 16; ++k)
-                                umma_f16_ts(tmem + 256 + 128 * t, tmem + 128 * t + 8 * k, sw128_mnmajor_desc(va + k * 2048),
-                                            kPV, j > 0 || k > 0);
-                            umma_commit(o_done + t);
-                        }
-                        __syncwarp();
-                    }
-                    if (j + 1 < nb) qk(t, j + 1);
+                if (j >= nb) {
+                    pass(iv);
+                    if (j + 1 < nblk) pass(iv + 1);
+                    continue;
                 }
-                if (lane == 0 && ok) {
+                ok = wait(kv_full + sv, (uint32_t)(iv / kStages) & 1u) && (j + 1 >= nblk || k_there(j + 1)) &&
+                     wait(p_full + t, (uint32_t)j & 1u);
+                // the tiles take turns, so that one's products are not spread over both's time: the
+                // softmax that waits for them starts as early as it can, and the other one meanwhile
+                if (ok && (t ? j < nb_other : j > 0 && j - 1 < nb_other)) ok = wait(turn + t, (uint32_t)(t ? j : j - 1) & 1u);
+                if (!ok) break;
+                tc_fence_after();
+                if (lane == 0) {
+                    const uint64_t dvs = dv + sv * (kTile >> 4);
+                    #pragma unroll
+                    for (int k = 0; k < kPaKeys / 16; ++k)
+                        umma_f16_ts(tO, tS + 8 * k, dvs + k * (2048 >> 4), kPV, j > 0 || k > 0);
+                    umma_commit(o_done + t);
                     umma_commit(kv_empty + sv);
-                    if (j + 1 < nblk) umma_commit(kv_empty + (2 * j + 2) % kStages);
+                    if (j + 1 < nb) qk(j + 1);
+                    else if (j + 1 < nblk) mbar_arrive(kv_empty + (iv + 1) % kStages);
+                    mbar_arrive(turn + (t ^ 1));
                 }
                 __syncwarp();
             }
@@ -377,23 +451,37 @@ prompt_tc_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__ C
             if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
             tc_fence_after();
             uint32_t s[4][32];
-            #pragma unroll
-            for (int x = 0; x < 4; ++x) tmem_ld_32x32b_x32(tS + 32 * x, s[x]);
+            tmem_ld_32x32b_x32(tS, s[0]);
+            tmem_ld_32x32b_x32(tS + 32, s[1]);
             tmem_ld_wait();
-            if ((j + 1) * kPaKeys > clear) {
-                const int left = lim - j * kPaKeys;
-                #pragma unroll
-                for (int x = 0; x < 128; ++x)
-                    if (x >= left) s[x >> 5][x & 31] = 0xFF800000u;   // -inf
-            }
+            tmem_ready(s[0]);
+            tmem_ready(s[1]);
+            tmem_ld_32x32b_x32(tS + 64, s[2]);
+            tmem_ld_32x32b_x32(tS + 96, s[3]);
+            const bool masked = (j + 1) * kPaKeys > clear;
+            const int left = lim - j * kPaKeys;
             float mx[4];
             #pragma unroll
             for (int x = 0; x < 4; ++x) {
-                mx[x] = __uint_as_float(s[x][0]);
+                if (x == 2) {
+                    tmem_ld_wait();
+                    tmem_ready(s[2]);
+                    tmem_ready(s[3]);
+                }
+                if (masked) {
+                    #pragma unroll
+                    for (int y = 0; y < 32; ++y)
+                        if (32 * x + y >= left) s[x][y] = 0xFF800000u;   // -inf
+                }
+                float a0 = __uint_as_float(s[x][0]), a1 = __uint_as_float(s[x][1]);
                 #pragma unroll
-                for (int y = 1; y < 32; ++y) mx[x] = fmaxf(mx[x], __uint_as_float(s[x][y]));
+                for (int y = 2; y < 32; y += 4) {
+                    a0 = max3(a0, __uint_as_float(s[x][y]), __uint_as_float(s[x][y + 1]));
+                    if (y + 2 < 32) a1 = max3(a1, __uint_as_float(s[x][y + 2]), __uint_as_float(s[x][y + 3]));
+                }
+                mx[x] = fmaxf(a0, a1);
             }
-            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+            const float top = max3(mx[0], mx[1], fmaxf(mx[2], mx[3]));
             if (__any_sync(0xffffffffu, top > m + slack || (m == -INFINITY && top > m))) {
                 const float mn = fmaxf(m, top);
                 if (j > 0) {
@@ -408,6 +496,7 @@ prompt_tc_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__ C
                         uint32_t o[16];
                         tmem_ld_32x32b_x16(tO + 16 * x, o);
                         tmem_ld_wait();
+                        tmem_ready(o);
                         #pragma unroll
                         for (int y = 0; y < 16; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * alpha);
                         tmem_st_32x32b_x16(tO + 16 * x, o);
@@ -419,25 +508,34 @@ prompt_tc_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__ C
             const float mc = m == -INFINITY ? 0.f : -m * c;
             const float2 c2 = make_float2(c, c), mc2 = make_float2(mc, mc);
             float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-            #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                uint32_t p[32];
+            auto weights = [&](auto masked_tag) {
                 #pragma unroll
-                for (int x = 0; x < 32; ++x) {
-                    const int e = 64 * half + 2 * x;
-                    float2 v = fma2(make_float2(__uint_as_float(s[e >> 5][e & 31]), __uint_as_float(s[e >> 5][(e & 31) + 1])),
-                                    c2, mc2);
-                    v.x = ex2(v.x);
-                    v.y = ex2(v.y);
-                    sum[x & 1] = add2(sum[x & 1], v);
-                    p[x] = pack2<T>(v.x, v.y);
+                for (int half = 0; half < 2; ++half) {
+                    uint32_t p[32];
+                    #pragma unroll
+                    for (int x = 0; x < 32; ++x) {
+                        const int e = 64 * half + 2 * x;
+                        float2 v = fma2(make_float2(__uint_as_float(s[e >> 5][e & 31]), __uint_as_float(s[e >> 5][(e & 31) + 1])),
+                                        c2, mc2);
+                        // a masked weight has to be 0 exactly: those blocks take no polynomial
+                        if (!decltype(masked_tag)::value && (x & 7) < kPoly) {
+                            v = ex2_poly<!kBf16>(v);
+                        } else {
+                            v.x = ex2(v.x);
+                            v.y = ex2(v.y);
+                        }
+                        sum[x & 1] = add2(sum[x & 1], v);
+                        p[x] = pack2<T>(v.x, v.y);
+                    }
+                    tmem_st_32x32b_x32(tS + 32 * half, p);
                 }
-                tmem_st_32x32b_x32(tS + 32 * half, p);
-            }
+                tmem_st_wait();
+                tc_fence_before();
+                mbar_arrive(p_full + t);
+            };
+            if (masked) weights(std::true_type{});
+            else weights(std::false_type{});
             l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-            tmem_st_wait();
-            tc_fence_before();
-            mbar_arrive(p_full + t);
         }
         // ---- O / l
         if (ok && nb > 0) ok = mbar_wait(o_done + t, (uint32_t)(nb - 1) & 1u);
@@ -452,6 +550,7 @@ prompt_tc_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__ C
                 if (nb > 0) {
                     tmem_ld_32x32b_x32(tO + 32 * x, o);
                     tmem_ld_wait();
+                    tmem_ready(o);
                 }
                 if (!live) continue;
                 #pragma unroll

@@ -147,7 +147,7 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
 // usual widths with every channel turned, known to the compiler (0: any). kRows
 // rows a lane are loaded before the first is used.
 template <typename TI, typename TO, int D>
-__global__ void __launch_bounds__(kRopeThreads, 4)
+__global__ void __launch_bounds__(kRopeThreads, D ? 4 : 2)
 qk_norm_rope_kernel(const __grid_constant__ RopeArgs a, int gs_any) {
     __shared__ double turns[kMaxPairs];
     __shared__ unsigned char axis[kMaxPairs];
