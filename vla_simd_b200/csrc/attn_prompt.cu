@@ -11,11 +11,15 @@
 // the group) pairs, token-major: the keys of a group are loaded once for all of
 // its heads, and a causal tile spans 128 / group tokens, which keeps what the
 // mask throws away small. Warps: 0-3 and 4-7 the softmax of tile 0 and 1 (thread
-// = row = TMEM lane), 8 and 9 issue the matrix products of tile 0 and 1 (each
-// waits for its own tile alone: with one warp for both, the tiles ran in
-// lockstep, 4130 cycles a pair of blocks), 10 the TMA loads of a ring of K and V
-// tiles, 11 looks over the value tiles that are not seen in full. While one
-// tile's softmax runs, the tensor core has the other's products.
+// = row = TMEM lane), 8 and 9 issue the matrix products of tile 0 and 1, 10 the
+// TMA loads of a ring of K and V tiles, 11 looks over the value tiles that are
+// not seen in full.
+//
+// TMEM's 512 columns are full with two O tiles of 128 channels and 128 columns of
+// scores for each: as two buffers of 64 keys, so that the products of a buffer
+// run under the softmax of the other. (One buffer of 128 keys, the two tiles in
+// turn, left the tensor core idle for half the time: a block's softmax, 2000
+// cycles, and its products, 1400, followed one another.)
 //
 // m only follows the true maximum when it is more than 2^8 behind (P then stays
 // below 2^8, far inside bf16 and fp16): O is rescaled in TMEM that rarely, by
@@ -84,7 +88,8 @@ __device__ __noinline__ void prompt_row(const PromptArgs& a, int row, int head, 
         if (lane + 32 * x < a.d) out[lane + 32 * x] = from_f<T>(o[x] * inv);
 }
 
-constexpr int kPaThreads = 384, kPaRows = 128, kPaKeys = 128;
+constexpr int kPaThreads = 384, kPaRows = 128, kPaKeys = 128;   // keys of a ring tile
+constexpr int kPaStep = 64;                                     // keys of a step of the softmax
 // registers a thread: the softmax warpgroups take what the third one gives up
 constexpr int kPaRegsSoftmax = 208, kPaRegsRest = 88, kPaRegsAtLaunch = (2 * kPaRegsSoftmax + kPaRegsRest) / 3;
 constexpr uint32_t kPaBoxBytes = 128 * 128;   // 128 rows of 64 channels
@@ -219,10 +224,9 @@ prompt_tc_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__ C
     uint64_t* kv_full = q_full + 1;
     uint64_t* kv_empty = kv_full + kStages;
     uint64_t* v_raw = kv_empty + kStages;   // value tiles that warp 11 looks over first
-    uint64_t* s_full = v_raw + kStages;
-    uint64_t* p_full = s_full + 2;
-    uint64_t* turn = p_full + 2;
-    uint64_t* o_done = turn + 2;
+    uint64_t* s_full = v_raw + kStages;     // [tile][buffer]
+    uint64_t* p_full = s_full + 4;
+    uint64_t* o_done = p_full + 4;
     uint32_t* tslot = reinterpret_cast<uint32_t*>(o_done + 2);
     PromptJob* job = reinterpret_cast<PromptJob*>(tslot + 2);
 
@@ -237,12 +241,12 @@ prompt_tc_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__ C
             mbar_init(kv_empty + i, 2);
             mbar_init(v_raw + i, 1);
         }
-        for (int t = 0; t < 2; ++t) {
-            mbar_init(s_full + t, 1);
-            mbar_init(p_full + t, 128);
-            mbar_init(turn + t, 1);
-            mbar_init(o_done + t, 1);
+        for (int i = 0; i < 4; ++i) {
+            mbar_init(s_full + i, 1);
+            mbar_init(p_full + i, 4);
         }
+        mbar_init(o_done, 1);
+        mbar_init(o_done + 1, 1);
         fence_mbar_init();
         tma_prefetch_desc(&mq);
         tma_prefetch_desc(&mk);
@@ -300,6 +304,7 @@ prompt_tc_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__ C
     const int seq = job->seq;
     const int nblk0 = (job->keys[0] + kPaKeys - 1) / kPaKeys, nblk1 = (job->keys[1] + kPaKeys - 1) / kPaKeys;
     const int nblk = max(nblk0, nblk1);
+    const int nstep0 = (job->keys[0] + kPaStep - 1) / kPaStep, nstep1 = (job->keys[1] + kPaStep - 1) / kPaStep;
 
     if (warp >= 8) {
         regs_dec<kPaRegsRest>();
@@ -369,66 +374,56 @@ prompt_tc_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__ C
             }
         } else if (warp < 10 && nblk > 0) {
             // ---- matrix products of tile t; a ring stage is free when both warps are past it
-            const int t = warp - 8, nb = t ? nblk1 : nblk0;
+            const int t = warp - 8, ns = t ? nstep1 : nstep0, nb = t ? nblk1 : nblk0;
             constexpr uint32_t kPV = idesc_f16(kBf16, D, true, false);
-            const uint32_t kQK = a.negate ? idesc_f16(kBf16, kPaKeys, false, true) : idesc_f16(kBf16, kPaKeys, false, false);
+            const uint32_t kQK = a.negate ? idesc_f16(kBf16, kPaStep, false, true) : idesc_f16(kBf16, kPaStep, false, false);
             const uint64_t dq = sw128_kmajor_desc(smem_u32(sq + t * kTile)), dk = sw128_kmajor_desc(smem_u32(ring));
             const uint64_t dv = sw128_mnmajor_desc(smem_u32(ring));
             const uint32_t tS = tmem + 128 * t, tO = tmem + 256 + 128 * t;
             auto wait = [](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)) != 0; };
             bool ok = wait(q_full, 0);
-            auto k_there = [&](int j) { return wait(kv_full + 2 * j % kStages, (uint32_t)(2 * j / kStages) & 1u); };
-            auto qk = [&](int j) {   // one thread
-                const int st = 2 * j % kStages;
-                const uint64_t dks = dk + st * (kTile >> 4);
+            auto there = [&](int i) { return wait(kv_full + i % kStages, (uint32_t)(i / kStages) & 1u); };
+            // scores of step i (half of K tile i / 2) into buffer i % 2; one thread
+            auto qk = [&](int i) {
+                const int st = (i & ~1) % kStages;
+                const uint64_t dks = dk + ((st * kTile + (i & 1) * (kPaStep * 128)) >> 4);
                 #pragma unroll
                 for (int k = 0; k < D / 16; ++k) {   // 32 bytes a step, 64 channels a box
                     const int off = ((k >> 2) * kPaBoxBytes + (k & 3) * 32) >> 4;
-                    umma_f16_ss(tS, dq + off, dks + off, kQK, k > 0);
+                    umma_f16_ss(tS + kPaStep * (i & 1), dq + off, dks + off, kQK, k > 0);
                 }
-                umma_commit(s_full + t);
-                umma_commit(kv_empty + st);
+                umma_commit(s_full + 2 * t + (i & 1));
+                if ((i & 1) || i == ns - 1) umma_commit(kv_empty + st);
             };
-            // a tile without block i / 2 passes it on, once it is there (one arrival a round)
-            auto pass = [&](int i) {
-                ok = ok && wait(kv_full + i % kStages, (uint32_t)(i / kStages) & 1u);
-                if (ok && lane == 0) mbar_arrive(kv_empty + i % kStages);
-                __syncwarp();
-            };
-            if (nb > 0) {
-                ok = ok && k_there(0);
+            if (ns > 0 && ok) {
+                ok = there(0);
                 tc_fence_after();
-                if (ok && lane == 0) qk(0);
-                __syncwarp();
-            } else {
-                pass(0);
-            }
-            const int nb_other = t ? nblk0 : nblk1;
-            for (int j = 0; j < nblk && ok; ++j) {
-                const int iv = 2 * j + 1, sv = iv % kStages;
-                if (j >= nb) {
-                    pass(iv);
-                    if (j + 1 < nblk) pass(iv + 1);
-                    continue;
+                if (ok && lane == 0) {
+                    qk(0);
+                    if (ns > 1) qk(1);
                 }
-                ok = wait(kv_full + sv, (uint32_t)(iv / kStages) & 1u) && (j + 1 >= nblk || k_there(j + 1)) &&
-                     wait(p_full + t, (uint32_t)j & 1u);
-                // the tiles take turns, so that one's products are not spread over both's time: the
-                // softmax that waits for them starts as early as it can, and the other one meanwhile
-                if (ok && (t ? j < nb_other : j > 0 && j - 1 < nb_other)) ok = wait(turn + t, (uint32_t)(t ? j : j - 1) & 1u);
+                __syncwarp();
+            }
+            for (int i = 0; i < ns && ok; ++i) {
+                const int iv = 2 * (i >> 1) + 1, sv = iv % kStages, b = i & 1;
+                ok = (b || (there(iv) && (i + 2 >= ns || there(iv + 1)))) && wait(p_full + 2 * t + b, (uint32_t)(i >> 1) & 1u);
                 if (!ok) break;
                 tc_fence_after();
                 if (lane == 0) {
-                    const uint64_t dvs = dv + sv * (kTile >> 4);
+                    const uint64_t dvs = dv + ((sv * kTile + b * (kPaStep * 128)) >> 4);
                     #pragma unroll
-                    for (int k = 0; k < kPaKeys / 16; ++k)
-                        umma_f16_ts(tO, tS + 8 * k, dvs + k * (2048 >> 4), kPV, j > 0 || k > 0);
+                    for (int k = 0; k < kPaStep / 16; ++k)
+                        umma_f16_ts(tO, tS + kPaStep * b + 8 * k, dvs + k * (2048 >> 4), kPV, i > 0 || k > 0);
                     umma_commit(o_done + t);
-                    umma_commit(kv_empty + sv);
-                    if (j + 1 < nb) qk(j + 1);
-                    else if (j + 1 < nblk) mbar_arrive(kv_empty + (iv + 1) % kStages);
-                    mbar_arrive(turn + (t ^ 1));
+                    if (b || i == ns - 1) umma_commit(kv_empty + sv);
+                    if (i + 2 < ns) qk(i + 2);
                 }
+                __syncwarp();
+            }
+            // tiles of the ring that only the other one uses: passed on once they are there
+            for (int i = 2 * nb; i < 2 * nblk && ok; ++i) {
+                ok = there(i);
+                if (ok && lane == 0) mbar_arrive(kv_empty + i % kStages);
                 __syncwarp();
             }
         }
@@ -436,38 +431,32 @@ prompt_tc_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__ C
         regs_inc<kPaRegsSoftmax>();
         // ---- softmax: thread = row
         const int t = warp >> 2, r = tid & 127;
-        const int nb = t ? nblk1 : nblk0;
+        const int ns = t ? nstep1 : nstep0;
         const int rt = r / a.gp, rg = r - rt * a.gp;
         const bool live = rt < job->n_tok[t] && seq >= 0;
         const int lim = live ? prompt_limit(a, seq, job->tok[t] + rt, job->lq, job->lk) : 0;
-        const int clear = nb > 0 ? prompt_limit(a, seq, job->tok[t], job->lq, job->lk) : 0;   // fewest keys of the tile
+        const int clear = ns > 0 ? prompt_limit(a, seq, job->tok[t], job->lq, job->lk) : 0;   // fewest keys of the tile
         const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t tS = tmem + 128 * t + lane_base, tO = tmem + 256 + 128 * t + lane_base;
         const float c = a.scale_log2, slack = 8.0f / c;
         float m = -INFINITY, l = 0.f;
         bool ok = true;
-        for (int j = 0; j < nb; ++j) {
-            ok = mbar_wait(s_full + t, (uint32_t)j & 1u);
-            if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+        for (int i = 0; i < ns; ++i) {
+            const uint32_t tB = tS + kPaStep * (i & 1);
+            ok = __all_sync(0xffffffffu, mbar_wait(s_full + 2 * t + (i & 1), (uint32_t)(i >> 1) & 1u)) != 0;
+            if (!ok) break;
             tc_fence_after();
-            uint32_t s[4][32];
-            tmem_ld_32x32b_x32(tS, s[0]);
-            tmem_ld_32x32b_x32(tS + 32, s[1]);
+            uint32_t s[2][32];
+            tmem_ld_32x32b_x32(tB, s[0]);
+            tmem_ld_32x32b_x32(tB + 32, s[1]);
             tmem_ld_wait();
             tmem_ready(s[0]);
             tmem_ready(s[1]);
-            tmem_ld_32x32b_x32(tS + 64, s[2]);
-            tmem_ld_32x32b_x32(tS + 96, s[3]);
-            const bool masked = (j + 1) * kPaKeys > clear;
-            const int left = lim - j * kPaKeys;
-            float mx[4];
+            const bool masked = (i + 1) * kPaStep > clear;
+            const int left = lim - i * kPaStep;
+            float mx[2];
             #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                if (x == 2) {
-                    tmem_ld_wait();
-                    tmem_ready(s[2]);
-                    tmem_ready(s[3]);
-                }
+            for (int x = 0; x < 2; ++x) {
                 if (masked) {
                     #pragma unroll
                     for (int y = 0; y < 32; ++y)
@@ -481,13 +470,13 @@ prompt_tc_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__ C
                 }
                 mx[x] = fmaxf(a0, a1);
             }
-            const float top = max3(mx[0], mx[1], fmaxf(mx[2], mx[3]));
+            const float top = fmaxf(mx[0], mx[1]);
             if (__any_sync(0xffffffffu, top > m + slack || (m == -INFINITY && top > m))) {
                 const float mn = fmaxf(m, top);
-                if (j > 0) {
-                    // rescale O once the products so far are in
-                    ok = mbar_wait(o_done + t, (uint32_t)(j - 1) & 1u);
-                    if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+                if (i > 0) {
+                    // rescale O once the products so far are in (this step's are not issued before its P is there)
+                    ok = __all_sync(0xffffffffu, mbar_wait(o_done + t, (uint32_t)(i - 1) & 1u)) != 0;
+                    if (!ok) break;
                     tc_fence_after();
                     const float alpha = m == -INFINITY ? 0.f : ex2((m - mn) * c);
                     l *= alpha;
@@ -508,46 +497,44 @@ prompt_tc_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__ C
             const float mc = m == -INFINITY ? 0.f : -m * c;
             const float2 c2 = make_float2(c, c), mc2 = make_float2(mc, mc);
             float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+            uint32_t p[32];
             auto weights = [&](auto masked_tag) {
                 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    uint32_t p[32];
-                    #pragma unroll
-                    for (int x = 0; x < 32; ++x) {
-                        const int e = 64 * half + 2 * x;
-                        float2 v = fma2(make_float2(__uint_as_float(s[e >> 5][e & 31]), __uint_as_float(s[e >> 5][(e & 31) + 1])),
-                                        c2, mc2);
-                        // a masked weight has to be 0 exactly: those blocks take no polynomial
-                        if (!decltype(masked_tag)::value && (x & 7) < kPoly) {
-                            v = ex2_poly<!kBf16>(v);
-                        } else {
-                            v.x = ex2(v.x);
-                            v.y = ex2(v.y);
-                        }
-                        sum[x & 1] = add2(sum[x & 1], v);
-                        p[x] = pack2<T>(v.x, v.y);
+                for (int x = 0; x < 32; ++x) {
+                    const int e = 2 * x;
+                    float2 v = fma2(make_float2(__uint_as_float(s[e >> 5][e & 31]), __uint_as_float(s[e >> 5][(e & 31) + 1])),
+                                    c2, mc2);
+                    // a masked weight has to be 0 exactly: those blocks take no polynomial
+                    if (!decltype(masked_tag)::value && (x & 7) < kPoly) {
+                        v = ex2_poly<!kBf16>(v);
+                    } else {
+                        v.x = ex2(v.x);
+                        v.y = ex2(v.y);
                     }
-                    tmem_st_32x32b_x32(tS + 32 * half, p);
+                    sum[x & 1] = add2(sum[x & 1], v);
+                    p[x] = pack2<T>(v.x, v.y);
                 }
-                tmem_st_wait();
-                tc_fence_before();
-                mbar_arrive(p_full + t);
             };
             if (masked) weights(std::true_type{});
             else weights(std::false_type{});
+            tmem_st_32x32b_x32(tB, p);
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(p_full + 2 * t + (i & 1));
             l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
         }
         // ---- O / l
-        if (ok && nb > 0) ok = mbar_wait(o_done + t, (uint32_t)(nb - 1) & 1u);
+        if (ok && ns > 0) ok = mbar_wait(o_done + t, (uint32_t)(ns - 1) & 1u);
         ok = __all_sync(0xffffffffu, ok);
         if (ok) {
             tc_fence_after();
-            const float inv = nb > 0 && l != 0.f ? 1.0f / l : 0.f;
+            const float inv = ns > 0 && l != 0.f ? 1.0f / l : 0.f;
             T* out = static_cast<T*>(a.out) + ((long long)(job->q0 + job->tok[t] + rt) * a.n_q + head0 + rg) * a.d;
             #pragma unroll 1
             for (int x = 0; x < D / 32; ++x) {
                 uint32_t o[32];
-                if (nb > 0) {
+                if (ns > 0) {
                     tmem_ld_32x32b_x32(tO + 32 * x, o);
                     tmem_ld_wait();
                     tmem_ready(o);
@@ -557,7 +544,7 @@ prompt_tc_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__ C
                 for (int y = 0; y < 4; ++y) {
                     if (32 * x + 8 * y >= a.d) break;
                     uint4 w = make_uint4(0u, 0u, 0u, 0u);
-                    if (nb > 0 && lim > 0) {
+                    if (ns > 0 && lim > 0) {
                         w.x = pack2<T>(__uint_as_float(o[8 * y]) * inv, __uint_as_float(o[8 * y + 1]) * inv);
                         w.y = pack2<T>(__uint_as_float(o[8 * y + 2]) * inv, __uint_as_float(o[8 * y + 3]) * inv);
                         w.z = pack2<T>(__uint_as_float(o[8 * y + 4]) * inv, __uint_as_float(o[8 * y + 5]) * inv);
@@ -566,7 +553,7 @@ prompt_tc_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__ C
                     *reinterpret_cast<uint4*>(out + 32 * x + 8 * y) = w;
                 }
             }
-            if (nb > 0 && *reinterpret_cast<volatile int*>(&job->bad)) {
+            if (ns > 0 && *reinterpret_cast<volatile int*>(&job->bad)) {
                 __syncwarp();
                 for (int x = 0; x < 32; ++x) {
                     const int xr = __shfl_sync(0xffffffffu, rt, x), xg = __shfl_sync(0xffffffffu, rg, x);
