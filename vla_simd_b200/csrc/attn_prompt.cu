@@ -145,6 +145,12 @@ __device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+__device__ __forceinline__ bool elect_one() {   // one lane of a converged warp
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
+
 template <int N>
 __device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(N)); }
 template <int N>
@@ -222,12 +228,13 @@ prompt_tc_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__ C
     uint8_t* ring = sm + 2 * kTile;
     uint64_t* q_full = reinterpret_cast<uint64_t*>(ring + kStages * kTile);
     uint64_t* kv_full = q_full + 1;
-    uint64_t* kv_empty = kv_full + kStages;
-    uint64_t* v_raw = kv_empty + kStages;   // value tiles that warp 11 looks over first
-    uint64_t* s_full = v_raw + kStages;     // [tile][buffer]
+    uint64_t* v_raw = kv_full + kStages;    // value tiles that warp 11 looks over first
+    uint64_t* kv_empty = v_raw + kStages;   // [pair % 4]
+    uint64_t* s_full = kv_empty + 4;        // [tile][buffer]
     uint64_t* p_full = s_full + 4;
-    uint64_t* o_done = p_full + 4;
-    uint32_t* tslot = reinterpret_cast<uint32_t*>(o_done + 2);
+    uint64_t* o_done = p_full + 4;          // the last output product of a tile
+    uint64_t* o_prev = o_done + 2;          // the one before it
+    uint32_t* tslot = reinterpret_cast<uint32_t*>(o_prev + 2);
     PromptJob* job = reinterpret_cast<PromptJob*>(tslot + 2);
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -238,15 +245,17 @@ prompt_tc_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__ C
         mbar_init(q_full, 1);
         for (int i = 0; i < kStages; ++i) {
             mbar_init(kv_full + i, 1);
-            mbar_init(kv_empty + i, 2);
             mbar_init(v_raw + i, 1);
         }
         for (int i = 0; i < 4; ++i) {
             mbar_init(s_full + i, 1);
             mbar_init(p_full + i, 4);
+            mbar_init(kv_empty + i, 2);
         }
-        mbar_init(o_done, 1);
-        mbar_init(o_done + 1, 1);
+        for (int t = 0; t < 2; ++t) {
+            mbar_init(o_done + t, 1);
+            mbar_init(o_prev + t, 1);
+        }
         fence_mbar_init();
         tma_prefetch_desc(&mq);
         tma_prefetch_desc(&mk);
@@ -306,13 +315,14 @@ prompt_tc_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__ C
     const int nblk = max(nblk0, nblk1);
     const int nstep0 = (job->keys[0] + kPaStep - 1) / kPaStep, nstep1 = (job->keys[1] + kPaStep - 1) / kPaStep;
 
+    // the fewest keys any row here sees: past them some weights are masked to 0
+    const int clear_all = nblk > 0 ? prompt_limit(a, seq, job->n_tok[0] > 0 ? job->tok[0] : job->tok[1], job->lq, job->lk) : 0;
+    const int masked0 = clear_all / kPaKeys;   // the first block that is not seen in full
+    // masked value blocks go round the ring's stages with this period
+    constexpr int kPeriod = kStages % 2 ? kStages : kStages / 2;
+
     if (warp >= 8) {
         regs_dec<kPaRegsRest>();
-        // the fewest keys any row here sees: past them some weights are masked to 0
-        const int clear_all = nblk > 0 ? prompt_limit(a, seq, job->n_tok[0] > 0 ? job->tok[0] : job->tok[1], job->lq, job->lk) : 0;
-        const int masked0 = clear_all / kPaKeys;   // the first block that is not seen in full
-        // masked value blocks go round the ring's stages with this period
-        constexpr int kPeriod = kStages % 2 ? kStages : kStages / 2;
         if (warp == 10 && nblk > 0) {
             // ---- loads: Q tiles, then K and V of each block through the ring
             if (lane == 0) {
@@ -324,7 +334,10 @@ prompt_tc_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__ C
                 int i = 0;
                 for (; i < 2 * nblk; ++i) {
                     const int st = i % kStages;
-                    if (i >= kStages && !mbar_wait(kv_empty + st, (uint32_t)(i / kStages - 1) & 1u)) break;
+                    if (i >= kStages) {
+                        const int old = (i - kStages + 1) >> 1;   // the pair of the tile that was here
+                        if (!mbar_wait(kv_empty + (old & 3), (uint32_t)(old >> 2) & 1u)) break;
+                    }
                     uint64_t* bar = (i & 1) && (i >> 1) >= masked0 ? v_raw + st : kv_full + st;
                     mbar_arrive_expect_tx(bar, kTile);
                     for (int c = 0; c < kCB; ++c)
@@ -373,16 +386,17 @@ prompt_tc_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__ C
                 if (lane == 0) mbar_arrive(kv_full + st);
             }
         } else if (warp < 10 && nblk > 0) {
-            // ---- matrix products of tile t; a ring stage is free when both warps are past it
-            const int t = warp - 8, ns = t ? nstep1 : nstep0, nb = t ? nblk1 : nblk0;
+            // ---- matrix products of tile t, by one elected thread. It has to be elect.sync around the whole
+            // loop: the operands of a product are uniform registers, and behind `lane == 0` inside the loop
+            // each product took 50 to 90 cycles to issue (64 to run). One commit a step: that of the scores
+            // of step i + 2 also tells that the output product of step i, issued before them, is done.
+            const int t = warp - 8, ns = t ? nstep1 : nstep0;
             constexpr uint32_t kPV = idesc_f16(kBf16, D, true, false);
             const uint32_t kQK = a.negate ? idesc_f16(kBf16, kPaStep, false, true) : idesc_f16(kBf16, kPaStep, false, false);
             const uint64_t dq = sw128_kmajor_desc(smem_u32(sq + t * kTile)), dk = sw128_kmajor_desc(smem_u32(ring));
             const uint64_t dv = sw128_mnmajor_desc(smem_u32(ring));
             const uint32_t tS = tmem + 128 * t, tO = tmem + 256 + 128 * t;
-            auto wait = [](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)) != 0; };
-            bool ok = wait(q_full, 0);
-            auto there = [&](int i) { return wait(kv_full + i % kStages, (uint32_t)(i / kStages) & 1u); };
+            auto there = [&](int i) { return mbar_wait(kv_full + i % kStages, (uint32_t)(i / kStages) & 1u); };
             // scores of step i (half of K tile i / 2) into buffer i % 2; one thread
             auto qk = [&](int i) {
                 const int st = (i & ~1) % kStages;
@@ -393,39 +407,27 @@ prompt_tc_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__ C
                     umma_f16_ss(tS + kPaStep * (i & 1), dq + off, dks + off, kQK, k > 0);
                 }
                 umma_commit(s_full + 2 * t + (i & 1));
-                if ((i & 1) || i == ns - 1) umma_commit(kv_empty + st);
             };
-            if (ns > 0 && ok) {
-                ok = there(0);
+            if (elect_one()) {
+                bool ok = ns > 0 && mbar_wait(q_full, 0) && there(0);
                 tc_fence_after();
-                if (ok && lane == 0) {
-                    qk(0);
-                    if (ns > 1) qk(1);
-                }
-                __syncwarp();
-            }
-            for (int i = 0; i < ns && ok; ++i) {
-                const int iv = 2 * (i >> 1) + 1, sv = iv % kStages, b = i & 1;
-                ok = (b || (there(iv) && (i + 2 >= ns || there(iv + 1)))) && wait(p_full + 2 * t + b, (uint32_t)(i >> 1) & 1u);
-                if (!ok) break;
-                tc_fence_after();
-                if (lane == 0) {
+                if (ok) qk(0);
+                if (ok && ns > 1) qk(1);
+                for (int i = 0; i < ns && ok; ++i) {
+                    const int iv = 2 * (i >> 1) + 1, sv = iv % kStages, b = i & 1;
+                    ok = (b || (there(iv) && (i + 2 >= ns || there(iv + 1)))) &&
+                         mbar_wait(p_full + 2 * t + b, (uint32_t)(i >> 1) & 1u);
+                    if (!ok) break;
+                    tc_fence_after();
                     const uint64_t dvs = dv + ((sv * kTile + b * (kPaStep * 128)) >> 4);
                     #pragma unroll
                     for (int k = 0; k < kPaStep / 16; ++k)
                         umma_f16_ts(tO, tS + kPaStep * b + 8 * k, dvs + k * (2048 >> 4), kPV, i > 0 || k > 0);
-                    umma_commit(o_done + t);
-                    if (b || i == ns - 1) umma_commit(kv_empty + sv);
                     if (i + 2 < ns) qk(i + 2);
+                    else umma_commit((i == ns - 1 ? o_done : o_prev) + t);
                 }
-                __syncwarp();
             }
-            // tiles of the ring that only the other one uses: passed on once they are there
-            for (int i = 2 * nb; i < 2 * nblk && ok; ++i) {
-                ok = there(i);
-                if (ok && lane == 0) mbar_arrive(kv_empty + i % kStages);
-                __syncwarp();
-            }
+            __syncwarp();
         }
     } else {
         regs_inc<kPaRegsSoftmax>();
@@ -441,11 +443,18 @@ prompt_tc_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__ C
         const float c = a.scale_log2, slack = 8.0f / c;
         float m = -INFINITY, l = 0.f;
         bool ok = true;
+        // the ring is freed in pairs: K tile 0, then p: V tile p - 1 and K tile p. When the scores of step 2 p +
+        // 1 are in, this tile's products with pair p are done.
+        int freed = 0;
         for (int i = 0; i < ns; ++i) {
             const uint32_t tB = tS + kPaStep * (i & 1);
             ok = __all_sync(0xffffffffu, mbar_wait(s_full + 2 * t + (i & 1), (uint32_t)(i >> 1) & 1u)) != 0;
             if (!ok) break;
             tc_fence_after();
+            if (i & 1) {
+                if (r == 0) mbar_arrive(kv_empty + (freed & 3));
+                ++freed;
+            }
             uint32_t s[2][32];
             tmem_ld_32x32b_x32(tB, s[0]);
             tmem_ld_32x32b_x32(tB + 32, s[1]);
@@ -475,7 +484,8 @@ prompt_tc_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__ C
                 const float mn = fmaxf(m, top);
                 if (i > 0) {
                     // rescale O once the products so far are in (this step's are not issued before its P is there)
-                    ok = __all_sync(0xffffffffu, mbar_wait(o_done + t, (uint32_t)(i - 1) & 1u)) != 0;
+                    ok = __all_sync(0xffffffffu, i + 1 < ns ? mbar_wait(s_full + 2 * t + ((i + 1) & 1), (uint32_t)((i + 1) >> 1) & 1u)
+                                                            : mbar_wait(o_prev + t, 0)) != 0;
                     if (!ok) break;
                     tc_fence_after();
                     const float alpha = m == -INFINITY ? 0.f : ex2((m - mn) * c);
@@ -525,7 +535,16 @@ prompt_tc_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__ C
             l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
         }
         // ---- O / l
-        if (ok && ns > 0) ok = mbar_wait(o_done + t, (uint32_t)(ns - 1) & 1u);
+        if (ok && ns > 0) ok = mbar_wait(o_done + t, 0);
+        ok = __all_sync(0xffffffffu, ok);
+        // the rest of the ring's tiles, and those that only the other tile uses, once they are there
+        if (ok && r == 0)
+            for (; freed <= nblk && nblk > 0; ++freed) {
+                const int first = max(2 * freed - 1, 0), last = min(2 * freed, 2 * nblk - 1);
+                for (int x = first; x <= last && ok; ++x) ok = mbar_wait(kv_full + x % kStages, (uint32_t)(x / kStages) & 1u);
+                if (!ok) break;
+                mbar_arrive(kv_empty + (freed & 3));
+            }
         ok = __all_sync(0xffffffffu, ok);
         if (ok) {
             tc_fence_after();
