@@ -28,6 +28,7 @@
 #include "launch.cuh"
 #include "sm100.cuh"
 
+#include <algorithm>
 #include <atomic>
 #include <climits>
 #include <type_traits>
@@ -618,14 +619,19 @@ cudaError_t kv4_launch(const Kv4AttDev& p, dim3 grid, cudaStream_t st) {
     return launch_k(kv4_attention_kernel<NG, T>, grid, dim3(kKaThreads), ka_smem<NG>(), st, p);
 }
 
-// Keys a CTA takes: as many chunks as fill the SMs about four times over, none
-// shorter than one tile of each warp.
+// Keys a CTA takes. Three CTAs are resident on an SM: chunks down to a tile of
+// each warp fill one wave of them (latency: one sequence of 1021 tokens, 5 heads:
+// 6.9 us in 8 chunks); beyond that they only even out the tail, which pays down to
+// chunks of about 900 keys (16 sequences of up to 8192, 8 heads: 26 us in 10
+// chunks of 896, 30 in 5, 29 in 19) and not at 128 (8 sequences of 256 with 19
+// row tiles: 12 us whole, 17 in two).
 int kv4_chunk(int batch, int row_ctas, long long max_len) {
-    const long long tile = (long long)kKaTile * kKaWarps;
-    long long want = (148ll * 8 + (long long)batch * row_ctas - 1) / ((long long)batch * row_ctas);
-    long long chunk = (max_len + want - 1) / want;
-    chunk = (chunk + tile - 1) / tile * tile;
-    return (int)(chunk < tile ? tile : chunk);
+    const long long tile = (long long)kKaTile * kKaWarps, ctas = (long long)batch * row_ctas;
+    const long long fill = std::min((148 * 3 + ctas - 1) / ctas, max_len / tile);
+    const long long even = std::min((148 * 8 + ctas - 1) / ctas, max_len / 896);
+    const long long want = std::max({fill, even, 1ll});
+    const long long chunk = (max_len + want - 1) / want;
+    return (int)std::max((chunk + tile - 1) / tile * tile, tile);
 }
 
 }  // namespace

@@ -205,9 +205,9 @@ __device__ __forceinline__ float2 ex2_poly(float2 x) {
     return p;
 }
 
-#ifndef PA_POLY
-#define PA_POLY 0
-#endif
+// of 8 pairs of weights, how many the FMA pipe makes (0: 1870 us, 2: 1842, 3: 1815, 4: 1836 at 16384 tokens, 32
+// heads over 8 of 128: the SFUs alone are as long as the tensor core, the polynomial costs issue slots)
+constexpr int kPaPoly = 3;
 
 // What a CTA works on: tile t has rows of queries [tok[t], tok[t] + n_tok[t])
 // of the sequence and sees the first keys[t] of its lk keys.
@@ -220,7 +220,7 @@ __global__ void __launch_bounds__(kPaThreads, 1)
 prompt_tc_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__ CUtensorMap mq,
                  const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv) {
     constexpr bool kBf16 = sizeof(T) == 2 && !std::is_same<T, __half>::value;
-    constexpr int kStages = pa_stages(D), kCB = D / 64, kPoly = PA_POLY;
+    constexpr int kStages = pa_stages(D), kCB = D / 64, kPoly = kPaPoly;
     constexpr uint32_t kTile = kCB * kPaBoxBytes;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* sm = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
