@@ -215,6 +215,17 @@ def test_prompt_large_scores(dtype, d):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("nq,nkv,d", [(2, 1, 128), (3, 1, 64)])
+def test_prompt_of_many_ring_rounds(dtype, nq, nkv, d):
+    g = gen(17)
+    T = 3001
+    q, k, v = randn(g, T, nq, d, dtype=dtype), randn(g, T, nkv, d, dtype=dtype), randn(g, T, nkv, d, dtype=dtype)
+    check_prompt(q[:300], k, v, [300], [T])
+    check_prompt(q, k, v, [T], [T], causal=False)
+    check_prompt(q, k, v, [T - 64, 64], [T - 64, 64], prefix=[1500, 10])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
 def test_prompt_strides(dtype):
     g = gen(9)
     T, nq, nkv, d = 150, 6, 2, 64
