@@ -363,22 +363,22 @@ prompt_tc_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__ C
                 if (!__all_sync(0xffffffffu, mbar_wait(v_raw + st, (uint32_t)((j - masked0) / kPeriod) & 1u))) break;
                 uint8_t* vt = ring + st * kTile;
                 const int valid = min(job->lk - j * kPaKeys, kPaKeys);
+                // an infinity or a NaN has all exponent bits: the largest magnitude, as whole numbers, tells
                 constexpr uint32_t kExp = kBf16 ? 0x7F80u : 0x7C00u;
-                bool bad = false;
-                for (int c = 0; c < kCB; ++c)
+                const int seen = max(clear_all - j * kPaKeys, 0);   // keys in front that every row sees
+                uint32_t big = 0;
+                for (int c = 0; c < kCB; ++c) {
+                    uint4* tile = reinterpret_cast<uint4*>(vt + c * kPaBoxBytes);   // 8 to a key
                     #pragma unroll 8
-                    for (int x = lane; x < (int)kPaBoxBytes / 16; x += 32) {
-                        uint4* p = reinterpret_cast<uint4*>(vt + c * kPaBoxBytes) + x;
-                        if (x >= valid * 8) {
-                            *p = make_uint4(0u, 0u, 0u, 0u);
-                        } else {
-                            const uint4 w = *p;
-                            const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
-                            #pragma unroll
-                            for (int y = 0; y < 4; ++y)
-                                bad |= (ws[y] & kExp) == kExp || (ws[y] >> 16 & kExp) == kExp;
-                        }
+                    for (int x = seen * 8 + lane; x < valid * 8; x += 32) {
+                        const uint4 w = tile[x];
+                        big = __vmaxu2(__vmaxu2(big, w.x & 0x7FFF7FFFu), __vmaxu2(w.y & 0x7FFF7FFFu, w.z & 0x7FFF7FFFu));
+                        big = __vmaxu2(big, w.w & 0x7FFF7FFFu);
                     }
+                    #pragma unroll 4
+                    for (int x = valid * 8 + lane; x < kPaKeys * 8; x += 32) tile[x] = make_uint4(0u, 0u, 0u, 0u);
+                }
+                const bool bad = (big & 0xFFFFu) >= kExp || big >> 16 >= kExp;
                 if (bad) job->bad = 1;
                 __threadfence_block();
                 fence_proxy_async_smem();
