@@ -266,13 +266,16 @@ prompt_tc_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__ C
     if (warp == 0) {
         // the sequence this CTA's pair of tiles lies in: pairs are numbered by
         // sequence, and within one from its end, the rows with the most keys first
-        int want = blockIdx.x / head_blocks, found = -1, at = 0;
+        int want = blockIdx.x / head_blocks, found = -1, at = 0, q0 = 0, lq = 0, k0 = 0, lk = 0;
         for (int s0 = 0; s0 < a.n_seq && found < 0; s0 += 32) {
             const int s = s0 + lane;
-            int n = 0;
+            int n = 0, qa = 0, qb = 0, ka = 0, kb = 0;
             if (s < a.n_seq) {
-                const int lo = min(max(a.cu_q[s], 0), a.total_q), hi = min(max(a.cu_q[s + 1], lo), a.total_q);
-                n = (hi - lo + 2 * a.tile_tok - 1) / (2 * a.tile_tok);
+                qa = min(max(a.cu_q[s], 0), a.total_q);
+                qb = min(max(a.cu_q[s + 1], qa), a.total_q);
+                ka = min(max(a.cu_k[s], 0), a.total_k);
+                kb = min(max(a.cu_k[s + 1], ka), a.total_k);
+                n = (qb - qa + 2 * a.tile_tok - 1) / (2 * a.tile_tok);
             }
             int sum = n;
             for (int o = 1; o < 32; o <<= 1) {
@@ -284,6 +287,10 @@ prompt_tc_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__ C
                 const int l = __ffs(hit) - 1;
                 found = s0 + l;
                 at = __shfl_sync(0xffffffffu, sum, l) - 1 - want;   // pairs after this one
+                q0 = __shfl_sync(0xffffffffu, qa, l);
+                lq = __shfl_sync(0xffffffffu, qb, l) - q0;
+                k0 = __shfl_sync(0xffffffffu, ka, l);
+                lk = __shfl_sync(0xffffffffu, kb, l) - k0;
             } else {
                 want -= __shfl_sync(0xffffffffu, sum, 31);
             }
@@ -292,10 +299,10 @@ prompt_tc_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__ C
             PromptJob j = {};
             j.seq = found;
             if (found >= 0) {
-                j.q0 = min(max(a.cu_q[found], 0), a.total_q);
-                j.lq = min(max(a.cu_q[found + 1], j.q0), a.total_q) - j.q0;
-                j.k0 = min(max(a.cu_k[found], 0), a.total_k);
-                j.lk = min(max(a.cu_k[found + 1], j.k0), a.total_k) - j.k0;
+                j.q0 = q0;
+                j.lq = lq;
+                j.k0 = k0;
+                j.lk = lk;
                 for (int t = 0; t < 2; ++t) {
                     j.tok[t] = (2 * at + t) * a.tile_tok;
                     j.n_tok[t] = min(max(j.lq - j.tok[t], 0), a.tile_tok);
@@ -549,7 +556,11 @@ prompt_tc_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__ C
         if (ok) {
             tc_fence_after();
             const float inv = ns > 0 && l != 0.f ? 1.0f / l : 0.f;
-            T* out = static_cast<T*>(a.out) + ((long long)(job->q0 + job->tok[t] + rt) * a.n_q + head0 + rg) * a.d;
+            // Through the tile of Q, which no product reads any more, each warp its own 32 rows, so that a
+            // store writes whole rows (thread by thread, 16 bytes of 32 rows at a time, the stores took
+            // longer than a block). Chunk c of a row lies at c ^ row.
+            constexpr int kChunks = D / 8;
+            uint4* stage = reinterpret_cast<uint4*>(sq + t * kTile) + (warp & 3) * 32 * kChunks;
             #pragma unroll 1
             for (int x = 0; x < D / 32; ++x) {
                 uint32_t o[32];
@@ -558,10 +569,8 @@ prompt_tc_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__ C
                     tmem_ld_wait();
                     tmem_ready(o);
                 }
-                if (!live) continue;
                 #pragma unroll
                 for (int y = 0; y < 4; ++y) {
-                    if (32 * x + 8 * y >= a.d) break;
                     uint4 w = make_uint4(0u, 0u, 0u, 0u);
                     if (ns > 0 && lim > 0) {
                         w.x = pack2<T>(__uint_as_float(o[8 * y]) * inv, __uint_as_float(o[8 * y + 1]) * inv);
@@ -569,9 +578,21 @@ prompt_tc_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__ C
                         w.z = pack2<T>(__uint_as_float(o[8 * y + 4]) * inv, __uint_as_float(o[8 * y + 5]) * inv);
                         w.w = pack2<T>(__uint_as_float(o[8 * y + 6]) * inv, __uint_as_float(o[8 * y + 7]) * inv);
                     }
-                    *reinterpret_cast<uint4*>(out + 32 * x + 8 * y) = w;
+                    stage[lane * kChunks + ((4 * x + y) ^ (lane & (kChunks - 1)))] = w;
                 }
             }
+            __syncwarp();
+            const long long to = live ? ((long long)(job->q0 + job->tok[t] + rt) * a.n_q + head0 + rg) * a.d : -1;
+            constexpr int kRowsAtOnce = 32 / kChunks;
+            const int ch = lane % kChunks;
+            #pragma unroll 4
+            for (int x = 0; x < 32; x += kRowsAtOnce) {
+                const int row = x + lane / kChunks;
+                const long long at = __shfl_sync(0xffffffffu, to, row);
+                if (at >= 0 && 8 * ch < a.d)
+                    *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + at + 8 * ch) = stage[row * kChunks + (ch ^ (row & (kChunks - 1)))];
+            }
+            __syncwarp();
             if (ns > 0 && *reinterpret_cast<volatile int*>(&job->bad)) {
                 __syncwarp();
                 for (int x = 0; x < 32; ++x) {
