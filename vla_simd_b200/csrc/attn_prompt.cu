@@ -3,9 +3,12 @@
 //
 // One pass over the keys with the running maximum m and sum l of a softmax:
 //   S = Q K^T;  P = 2^(c (S - m)), c = scale log2(e);  l += rowsum P;  O += P V
-// both products on tcgen05 (128 x 128 x D, accumulators in TMEM), P written back
-// over S's columns as the A operand of the second one, so scores and weights
-// never leave the SM.
+// both products on tcgen05 (128 x 64 x D and 128 x D x 64, accumulators in TMEM),
+// P written back over S's columns as the A operand of the second one, so scores
+// and weights never leave the SM. 16384 tokens, 32 heads over 8 of 128, causal:
+// 1.82 ms, 1.2 PFLOP/s (72 % of a large library product's rate) where the power
+// cap allows; a step of 64 keys takes the two tiles 1750 cycles, the tensor core
+// 1400 of them, the rest is the softmax's instruction latency.
 //
 // A CTA has two 128-row tiles of one key head. A tile's rows are (query, head of
 // the group) pairs, token-major: the keys of a group are loaded once for all of
