@@ -27,6 +27,10 @@
 // m only follows the true maximum when it is more than 2^8 behind (P then stays
 // below 2^8, far inside bf16 and fp16): O is rescaled in TMEM that rarely, by
 // the softmax threads themselves.
+//
+// A score that is NaN or +infinity makes its row NaN, and so do scores that are
+// -infinity throughout. The exponentials need not carry that (the polynomial
+// cannot): the row's maximum is taken so that a NaN stays, and l becomes NaN.
 #include "serve_ops.h"
 #include "gemm_i8.h"
 #include "launch.cuh"
@@ -77,14 +81,16 @@ __device__ __noinline__ void prompt_row(const PromptArgs& a, int row, int head, 
             if (lane + 32 * x < a.d) s = fmaf(q[x], to_f(kp[lane + 32 * x]), s);
         for (int y = 16; y > 0; y >>= 1) s += __shfl_xor_sync(0xffffffffu, s, y);
         s *= c;
-        const float mn = fmaxf(m, s), alpha = ex2(m - mn), w = ex2(s - mn);
+        const float mn = fmaxf(m, s);
+        // a score of -infinity weighs nothing; NaN and +infinity stay (inf - inf)
+        const float alpha = m == -INFINITY ? 1.f : ex2(m - mn), w = s == -INFINITY ? 0.f : ex2(s - mn);
         m = mn;
         l = fmaf(l, alpha, w);
         #pragma unroll
         for (int x = 0; x < 4; ++x)
             if (lane + 32 * x < a.d) o[x] = fmaf(o[x], alpha, w * to_f(vp[lane + 32 * x]));
     }
-    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    const float inv = lim > 0 ? 1.0f / l : 0.f;   // keys that all weigh nothing: 0 * infinity
     T* out = static_cast<T*>(a.out) + ((long long)row * a.n_q + head) * a.d;
     #pragma unroll
     for (int x = 0; x < 4; ++x)
@@ -165,12 +171,6 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
         : "=l"(reinterpret_cast<unsigned long long&>(d))
         : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
     return d;
-}
-
-__device__ __forceinline__ float max3(float a, float b, float c) {
-    float r;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-    return r;
 }
 
 // The registers of a tcgen05.ld are there once tmem_ld_wait() has returned: no
@@ -484,12 +484,14 @@ prompt_tc_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__ C
                 float a0 = __uint_as_float(s[x][0]), a1 = __uint_as_float(s[x][1]);
                 #pragma unroll
                 for (int y = 2; y < 32; y += 4) {
-                    a0 = max3(a0, __uint_as_float(s[x][y]), __uint_as_float(s[x][y + 1]));
-                    if (y + 2 < 32) a1 = max3(a1, __uint_as_float(s[x][y + 2]), __uint_as_float(s[x][y + 3]));
+                    a0 = max_nan(a0, __uint_as_float(s[x][y]), __uint_as_float(s[x][y + 1]));
+                    if (y + 2 < 32) a1 = max_nan(a1, __uint_as_float(s[x][y + 2]), __uint_as_float(s[x][y + 3]));
                 }
-                mx[x] = fmaxf(a0, a1);
+                mx[x] = max_nan(a0, a1, a1);
             }
-            const float top = fmaxf(mx[0], mx[1]);
+            const float top = max_nan(mx[0], mx[1], mx[1]);
+            // a seen score that is NaN or +infinity: from here on the row's sum, and with it the row, is NaN
+            if (!(top <= 3.402823466e38f)) l = __int_as_float(0x7fffffff);
             if (__any_sync(0xffffffffu, top > m + slack || (m == -INFINITY && top > m))) {
                 const float mn = fmaxf(m, top);
                 if (i > 0) {
@@ -558,7 +560,8 @@ prompt_tc_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__ C
         ok = __all_sync(0xffffffffu, ok);
         if (ok) {
             tc_fence_after();
-            const float inv = ns > 0 && l != 0.f ? 1.0f / l : 0.f;
+            // keys that all score -infinity leave no maximum: NaN, as 0 / 0 is
+            const float inv = lim == 0 ? 0.f : m == -INFINITY ? __int_as_float(0x7fffffff) : 1.0f / l;
             // Through the tile of Q, which no product reads any more, each warp its own 32 rows, so that a
             // store writes whole rows (thread by thread, 16 bytes of 32 rows at a time, the stores took
             // longer than a block). Chunk c of a row lies at c ^ row.
