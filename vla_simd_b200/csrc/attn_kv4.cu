@@ -24,6 +24,11 @@
 // Each warp has a ring of its own of 32-token tiles, filled by untiled bulk
 // copies: a block of 16 tokens of one head is contiguous, so the page table costs
 // one look-up per 20 * d bytes and the loads no registers.
+//
+// The running maximum passes over a NaN score; the weights and their sum do not.
+// A part (a warp's keys, a chunk's) whose sum is NaN joins the others with the
+// reference +infinity, which makes its row NaN; -infinity is left to parts that
+// saw no key.
 #include "serve_ops.h"
 #include "launch.cuh"
 #include "sm100.cuh"
@@ -527,10 +532,11 @@ kv4_attention_kernel(const __grid_constant__ Kv4AttDev p) {
         mine.min[2 * quad + 1][n] += mc[1];
     }
     if (n == 0) {
-        mine.sum[2 * quad] += mc[2];
-        mine.sum[2 * quad + 1] += mc[3];
-        mine.ref[2 * quad] = m0 == -INFINITY ? -INFINITY : ref0;
-        mine.ref[2 * quad + 1] = m1 == -INFINITY ? -INFINITY : ref1;
+        const float sum0 = mine.sum[2 * quad] + mc[2], sum1 = mine.sum[2 * quad + 1] + mc[3];
+        mine.sum[2 * quad] = sum0;
+        mine.sum[2 * quad + 1] = sum1;
+        mine.ref[2 * quad] = sum0 != sum0 ? INFINITY : m0 == -INFINITY ? -INFINITY : ref0;
+        mine.ref[2 * quad + 1] = sum1 != sum1 ? INFINITY : m1 == -INFINITY ? -INFINITY : ref1;
     }
     __syncwarp();
     #pragma unroll
@@ -552,9 +558,9 @@ kv4_attention_kernel(const __grid_constant__ Kv4AttDev p) {
     for (int w = 0; w < kKaWarps; ++w) rmax = fmaxf(rmax, red[w].ref[r]);
     float wt[kKaWarps], lsum = 0.f;
     #pragma unroll
-    for (int w = 0; w < kKaWarps; ++w) {
-        wt[w] = red[w].ref[r] == -INFINITY ? 0.f : ex2(red[w].ref[r] - rmax);
-        lsum = wt[w] == 0.f ? lsum : fmaf(red[w].sum[r], wt[w], lsum);
+    for (int w = 0; w < kKaWarps; ++w) {   // a warp that saw no key: the weight -1, left out
+        wt[w] = red[w].ref[r] == -INFINITY ? -1.f : ex2(red[w].ref[r] - rmax);
+        lsum = wt[w] < 0.f ? lsum : fmaf(red[w].sum[r], wt[w], lsum);
     }
     const int rq = rrow / p.group, rh = kvh * p.group + rrow % p.group;
     const long long out_row = ((long long)b * a.queries + rq) * a.n_q + rh;
@@ -565,7 +571,7 @@ kv4_attention_kernel(const __grid_constant__ Kv4AttDev p) {
     for (int c = rl; c < D; c += kLanes) {
         float v = 0.f;
         #pragma unroll
-        for (int w = 0; w < kKaWarps; ++w) v = wt[w] == 0.f ? v : fmaf(red[w].o[r][c], wt[w], v);
+        for (int w = 0; w < kKaWarps; ++w) v = wt[w] < 0.f ? v : fmaf(red[w].o[r][c], wt[w], v);
         if (direct) out[c] = from_f<T>(v * inv);
         else part[c] = v;
     }
