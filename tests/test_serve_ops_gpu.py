@@ -613,3 +613,13 @@ def test_c_refusals():
         assert decode(**bad) == VLA_ERR_ARG, bad
     assert decode() == 0
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("power", [-121, -117, -110, 105, 110, 120, 122])
+def test_kv4_attention_queries_of_any_size(dtype, power):
+    """Queries near the ends of their type, the scale as far the other way: scores of ordinary size."""
+    g = gen(18)
+    cache, table, kv = make_cache(g, [300], 2, 64, 64)
+    q = randn(g, 1, 1, 4, 64, dtype=dtype).clamp(-7.9, 7.9).double() * 2.0 ** power
+    check_decode(q.to(dtype), cache, table, kv, True, scale=2.0 ** (-power - 3))

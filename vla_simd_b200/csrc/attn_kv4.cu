@@ -253,7 +253,8 @@ kv4_attention_kernel(const __grid_constant__ Kv4AttDev p) {
             }
         amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
         amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-        const int e = amax > 0.f ? min(max((int)(__float_as_uint(amax) >> 23) - 127, -100), 100) : 0;
+        // every finite query (the powers below stay normal numbers, a subnormal one keeps its bits)
+        const int e = amax > 0.f ? min(max((int)(__float_as_uint(amax) >> 23) - 127, -117), 127) : 0;
         const float up = __uint_as_float((uint32_t)(127 + 9 - e) << 23);
         const float mul = a.scale * 1.4426950408889634f * __uint_as_float((uint32_t)(127 - 9 + e) << 23);
         mul0 = __shfl_sync(0xffffffffu, mul, 8 * quad);
