@@ -165,3 +165,20 @@ def test_cache_bad_keys_and_values_that_weigh_next_to_nothing(dtype):
     bad = v.clone()
     bad[[10, 3000], 0, 9] = math.nan         # 32 channels of a value, not the row
     assert check_cache_rows(q, k, bad) == 0
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("d", [64, 128])
+def test_prompt_rows_before_a_hidden_value_keep_their_bits(dtype, d):
+    """A NaN in a value that a whole tile of rows does not multiply changes none of its bits, in any run."""
+    g = gen(24)
+    T = 512
+    q, k, v = (randn(g, T, 8, d, dtype=dtype) for _ in range(3))
+    cu = torch.tensor([0, T], dtype=torch.int32, device="cuda")
+    clean = ops.prompt_attention(q, k, v, cu)
+    bad = v.clone()
+    bad[200], bad[T - 1] = math.nan, math.inf
+    first = ops.prompt_attention(q, k, bad, cu)
+    assert torch.equal(first[:128], clean[:128]) and first[200:].isnan().any(-1).all()
+    for _ in range(20):
+        assert torch.equal(ops.prompt_attention(q, k, bad, cu).nan_to_num(9.0), first.nan_to_num(9.0))

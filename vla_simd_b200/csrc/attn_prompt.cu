@@ -213,9 +213,10 @@ __device__ __forceinline__ float2 ex2_poly(float2 x) {
 constexpr int kPaPoly = 3;
 
 // What a CTA works on: tile t has rows of queries [tok[t], tok[t] + n_tok[t])
-// of the sequence and sees the first keys[t] of its lk keys.
+// of the sequence and sees the first keys[t] of its lk keys. bad[t]: a value that
+// the mask hides from some row, in a block that tile t multiplies, is not finite.
 struct PromptJob {
-    int seq, q0, lq, k0, lk, tok[2], n_tok[2], keys[2], bad;
+    int seq, q0, lq, k0, lk, tok[2], n_tok[2], keys[2], bad[2];
 };
 
 template <typename T, int D>
@@ -389,7 +390,9 @@ prompt_tc_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__ C
                     for (int x = valid * 8 + lane; x < kPaKeys * 8; x += 32) tile[x] = make_uint4(0u, 0u, 0u, 0u);
                 }
                 const bool bad = (big & 0xFFFFu) >= kExp || big >> 16 >= kExp;
-                if (bad) job->bad = 1;
+                // for the tiles that multiply this block alone: the end of their products comes after this
+                if (bad && j < nblk0) job->bad[0] = 1;
+                if (bad && j < nblk1) job->bad[1] = 1;
                 __threadfence_block();
                 fence_proxy_async_smem();
                 __syncwarp();
@@ -599,7 +602,7 @@ prompt_tc_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__ C
                     *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + at + 8 * ch) = stage[row * kChunks + (ch ^ (row & (kChunks - 1)))];
             }
             __syncwarp();
-            if (ns > 0 && *reinterpret_cast<volatile int*>(&job->bad)) {
+            if (ns > 0 && *reinterpret_cast<volatile int*>(&job->bad[t])) {
                 __syncwarp();
                 for (int x = 0; x < 32; ++x) {
                     const int xr = __shfl_sync(0xffffffffu, rt, x), xg = __shfl_sync(0xffffffffu, rg, x);
