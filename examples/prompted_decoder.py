@@ -43,10 +43,19 @@ class PromptedDecoder:
                        for _ in range(layers)]
         self.norm, self.head = ones, weight(vocab, hidden)
         pages = -(-max_tokens // page)
+        self.batch, self.room, self.longest = batch, pages * page, 0
         self.caches = [ops.kv4_cache(batch * pages, n_kv, d, page) for _ in range(layers)]
         self.table = torch.arange(batch * pages, dtype=torch.int32, device="cuda").view(batch, pages)
         self.lens = torch.zeros(batch, dtype=torch.int32, device="cuda")
         self.next_pos = torch.zeros(batch, dtype=torch.int32, device="cuda")
+
+    def need(self, tokens, sequences):
+        """Refuses sequences and lengths (known on the host) that the page table has no place for: an index past it
+        would stop the device."""
+        if sequences != self.batch:
+            raise ValueError(f"{sequences} sequences for a cache of {self.batch}")
+        if tokens > self.room:
+            raise ValueError(f"a sequence of {tokens} tokens does not fit the cache's {self.room}: raise max_tokens")
 
     def slots(self, seq, at):
         """Cache slots of positions `at` of sequences `seq`."""
@@ -71,6 +80,10 @@ class PromptedDecoder:
     def prompt(self, x, lens, pos, frames):
         """x [T, hidden]: the prompts' embeddings, one after another; lens: their lengths; pos [3, T]; frames
         [batch]: how many leading tokens of each are frames. Returns the logits after each prompt."""
+        if min(lens, default=0) < 1 or x.shape[0] != sum(lens) or pos.shape != (3, sum(lens)):
+            raise ValueError("x and pos have to hold the tokens of every prompt, at least one each")
+        self.need(max(lens), len(lens))
+        self.longest = max(lens)
         lens_t = torch.tensor(lens, device="cuda")
         cu = torch.nn.functional.pad(lens_t.cumsum(0), (1, 0)).int()
         seq = torch.repeat_interleave(torch.arange(len(lens), device="cuda"), lens_t)
@@ -84,6 +97,8 @@ class PromptedDecoder:
 
     def step(self, tokens):
         """One token for every sequence; returns the logits after it."""
+        self.need(self.longest + 1, tokens.numel())
+        self.longest += 1
         seq = torch.arange(tokens.numel(), device="cuda")
         slots = self.slots(seq, self.lens.long())
         self.lens += 1
@@ -109,9 +124,9 @@ def main():
     ap.add_argument("--tokens", type=int, default=16)
     a = ap.parse_args()
     shapes = [(2, 8, 8, 21), (1, 8, 8, 5), (3, 8, 8, 40), (0, 0, 0, 9)]   # frames, rows, columns, words
-    dec = PromptedDecoder(layers=a.layers, batch=len(shapes))
     pos = [prompt_positions(*s) for s in shapes]
     lens = [p.shape[1] for p in pos]
+    dec = PromptedDecoder(layers=a.layers, batch=len(shapes), max_tokens=max(1024, max(lens) + a.tokens))
     x = torch.randn(sum(lens), dec.hidden, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda")
     frames = torch.tensor([f * r * c for f, r, c, _ in shapes], dtype=torch.int32, device="cuda")
     logits = dec.prompt(x, lens, torch.cat(pos, 1).int().cuda(), frames)
