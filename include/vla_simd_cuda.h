@@ -294,12 +294,12 @@ VLA_API int32_t vla_cuda_kv4_read(const void* cache, int64_t n_pages, int32_t pa
 
 /* Attention of new tokens over the 4-bit cache: q [batch][queries][n_q]
  * heads (strides q_seq, q_tok, q_head), table [batch][table_ld] int32 page
- * indices of which the first max_pages may be used, lens [batch] int32 tokens in
- * the cache (clamped to max_pages * page). Query i of sequence b sees its first
- * lens[b] tokens, or with causal != 0 the first clamp(lens[b] - queries + 1 + i,
- * 0, lens[b]) (the new tokens are the last ones of the cache). out
- * [batch][queries][n_q][head_dim], same type as q (any); a query that sees
- * nothing gives zeros. A page index outside the cache is not read: its tokens
+ * indices of which the first max_pages (of at most 2^30 tokens) may be used, lens
+ * [batch] int32 tokens in the cache (clamped to max_pages * page). Query i of
+ * sequence b sees its first lens[b] tokens, or with causal != 0 the first
+ * clamp(lens[b] - queries + 1 + i, 0, lens[b]) (the new tokens are the last ones
+ * of the cache). out [batch][queries][n_q][head_dim], same type as q (any); a
+ * query that sees nothing gives zeros. A page index outside the cache is not read: its tokens
  * are left out and the device status word is set. Bytes of the cache past
  * lens[b] may hold anything. `ws`: workspace_bytes device bytes, 16-byte
  * aligned (NULL where that is 0); calls that may overlap on the GPU need

@@ -82,3 +82,19 @@ def test_sizes():
     assert size(1, 1, 32, 8, 128, 1, 128) == 0 and size(1, 1, 32, 8, 128, 0, 64) == 0 and size(1, 1, 3, 2, 64, 8, 64) == 0
     # (head_dim + 2) fp32 for each row and chunk
     assert size(1, 1, 32, 8, 128, 64, 128) % (4 * 130 * 32) == 0 and size(1, 1, 32, 8, 128, 64, 128) > 0
+
+
+@pytest.mark.parametrize("page", [16, 256])
+def test_decode_refuses_tables_whose_keys_pass_32_bits(page):
+    """A chunk past the last key of 2^31 would have no 32-bit number: at most 2^30 tokens a sequence."""
+    L = lib()
+    most = 2 ** 30 // page
+    size = L.vla_cuda_kv4_attention_workspace_bytes
+    assert size(1, 1, 2, 2, 64, most, page) > 0 and size(1, 1, 2, 2, 64, most + 1, page) == 0
+
+    def call(pages):   # batch 0: nothing is launched
+        return L.vla_cuda_kv4_attention(P, P, 128, 128, 64, 0, P, 64, page, P, pages, pages, P, 0, 1, 2, 2, 64, 0.1, 1, P, 0, None)
+
+    assert call(most) == 0
+    for pages in (most + 1, (2 ** 31 - 1) // page):
+        assert call(pages) == VLA_ERR_ARG

@@ -809,6 +809,9 @@ static bool kv4_ok(const void* cache, int64_t n_pages, int32_t page, int32_t n_k
            n_kv > 0 && n_kv <= 65535 && (head_dim == 64 || head_dim == 128) && n_pages <= INT32_MAX / page;
 }
 
+// tokens that one sequence's pages may span: twice that (a chunk past the end) is still an int32
+constexpr int64_t kKv4MaxTokens = int64_t(1) << 30;
+
 int64_t vla_cuda_kv4_block_bytes(int32_t head_dim) { return head_dim == 64 || head_dim == 128 ? 20 * head_dim : 0; }
 
 int32_t vla_cuda_kv4_append(void* cache, int64_t n_pages, int32_t page, const void* k, int64_t k_tok, int64_t k_head,
@@ -834,7 +837,7 @@ int32_t vla_cuda_kv4_read(const void* cache, int64_t n_pages, int32_t page, void
 
 uint64_t vla_cuda_kv4_attention_workspace_bytes(int32_t batch, int32_t queries, int32_t n_q, int32_t n_kv,
                                                 int32_t head_dim, int32_t max_pages, int32_t page) {
-    if (!heads_ok(n_q, n_kv) || max_pages <= 0 || page <= 0) return 0;
+    if (!heads_ok(n_q, n_kv) || max_pages <= 0 || page <= 0 || max_pages > kKv4MaxTokens / page) return 0;
     return vsb::kv4_attention_ws_bytes(batch, queries, n_q, n_kv, head_dim, (long long)max_pages * page);
 }
 
@@ -844,7 +847,7 @@ int32_t vla_cuda_kv4_attention(void* out, const void* q, int64_t q_seq, int64_t 
                                int32_t queries, int32_t n_q, int32_t n_kv, int32_t head_dim, float scale,
                                int32_t causal, void* ws, uint64_t ws_bytes, void* stream) {
     if (!kv4_ok(cache, n_pages, page, n_kv, head_dim) || !type_ok(type) || !heads_ok(n_q, n_kv) || batch < 0 ||
-        batch > 65535 || queries < 0 || max_pages < 0 || max_pages > INT32_MAX / page || table_ld < max_pages ||
+        batch > 65535 || queries < 0 || max_pages < 0 || max_pages > kKv4MaxTokens / page || table_ld < max_pages ||
         !std::isfinite(scale))
         return VLA_ERR_ARG;
     if (batch == 0 || queries == 0) return VLA_OK;
