@@ -249,8 +249,8 @@ VLA_API int32_t vla_cuda_qk_norm_rope(void* q_out, void* k_out, int32_t out_type
  * sees nothing gives zeros, and keys and values it does not see do not reach it
  * whatever they hold. Rows outside every sequence are not written. type F16 or
  * BF16 (weights are rounded to it for the product with v); head_dim a multiple
- * of 8, at most 128; addresses of q, k, v, out and the strides multiples of 16 bytes, the
- * strides positive. */
+ * of 8, at most 128; total_q and total_k at most 2^30; addresses of q, k, v, out
+ * and the strides multiples of 16 bytes, the strides positive. */
 VLA_API int32_t vla_cuda_prompt_attention(void* out, const void* q, int64_t q_tok, int64_t q_head,
                                           const void* k, int64_t k_tok, int64_t k_head,
                                           const void* v, int64_t v_tok, int64_t v_head, int32_t type,

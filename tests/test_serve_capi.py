@@ -98,3 +98,10 @@ def test_decode_refuses_tables_whose_keys_pass_32_bits(page):
     assert call(most) == 0
     for pages in (most + 1, (2 ** 31 - 1) // page):
         assert call(pages) == VLA_ERR_ARG
+
+
+def test_prompt_refuses_totals_past_32_bits():
+    """Rounded up to whole tiles, a total near 2^31 would be negative."""
+    for n in (2 ** 30 + 1, 2 ** 31 - 1):
+        assert prompt(lib(), tq=n, n_seq=0) == VLA_ERR_ARG and prompt(lib(), tk=n, n_seq=0) == VLA_ERR_ARG
+    assert prompt(lib(), tq=2 ** 30, tk=2 ** 30, n_seq=0) == 0   # no sequence: nothing is launched

@@ -55,7 +55,7 @@ struct PromptArgs {
 
 // keys that query i of a sequence of lq queries and lk keys sees: [0, limit)
 __device__ __forceinline__ int prompt_limit(const PromptArgs& a, int seq, int i, int lq, int lk) {
-    int lim = a.causal ? min(max(i + 1 + lk - lq, 0), lk) : lk;
+    int lim = a.causal ? min(max(lk - lq + i + 1, 0), lk) : lk;
     if (a.prefix) lim = max(lim, min(a.prefix[seq], lk));
     return lim;
 }

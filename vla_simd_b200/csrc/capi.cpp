@@ -793,7 +793,10 @@ int32_t vla_cuda_prompt_attention(void* out, const void* q, int64_t q_tok, int64
                                   const int32_t* cu_q, const int32_t* cu_k, const int32_t* prefix, int32_t n_seq,
                                   int32_t total_q, int32_t total_k, int32_t n_q, int32_t n_kv, int32_t head_dim,
                                   float scale, int32_t causal, void* stream) {
-    if ((type != VLA_TYPE_F16 && type != VLA_TYPE_BF16) || n_seq < 0 || total_q < 0 || total_k < 0 ||
+    // a tile of keys past the last one still has a 32-bit number
+    constexpr int32_t most = 1 << 30;
+    if ((type != VLA_TYPE_F16 && type != VLA_TYPE_BF16) || n_seq < 0 || total_q < 0 || total_k < 0 || total_q > most ||
+        total_k > most ||
         !heads_ok(n_q, n_kv) || head_dim <= 0 || head_dim > 128 || head_dim % 8 || !std::isfinite(scale))
         return VLA_ERR_ARG;
     if (total_q == 0 || n_seq == 0) return VLA_OK;
