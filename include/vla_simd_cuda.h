@@ -214,7 +214,8 @@ VLA_API int32_t vla_cuda_conv_transpose1d(float* out, const float* x, const floa
  * Heads are [tokens][heads][head_dim] with a token and a head stride in
  * elements (so q, k and v may be views of one projection) and contiguous
  * channels; outputs are contiguous. Element types are VLA_TYPE_*. A query head
- * h reads key head h / (n_q / n_kv). Sums, maxima and norms are 32-bit. */
+ * h reads key head h / (n_q / n_kv). Sums, maxima and norms are 32-bit; what
+ * else is rounded to fewer bits stands at each entry. */
 #define VLA_TYPE_F32   0
 #define VLA_TYPE_F16   1
 #define VLA_TYPE_BF16  2
@@ -247,10 +248,12 @@ VLA_API int32_t vla_cuda_qk_norm_rope(void* q_out, void* k_out, int32_t out_type
  * or NULL) at least min(prefix[s], lk), so that a prompt's frames see one
  * another. out [total_q][n_q][head_dim] = softmax(scale q.k) v; a query that
  * sees nothing gives zeros, and keys and values it does not see do not reach it
- * whatever they hold. Rows outside every sequence are not written. type F16 or
- * BF16 (weights are rounded to it for the product with v); head_dim a multiple
- * of 8, at most 128; total_q and total_k at most 2^30; addresses of q, k, v, out
- * and the strides multiples of 16 bytes, the strides positive. */
+ * whatever they hold. A score that is NaN or +infinity makes its row NaN, as do
+ * scores that are all -infinity. Rows outside every sequence are not written.
+ * type F16 or BF16: the weights are rounded to it for the product with v, and 3
+ * of 8 come from a polynomial good to 2^-18.5 (F16) or 2^-13.7 (BF16). head_dim
+ * a multiple of 8, at most 128; total_q and total_k at most 2^30; addresses of q,
+ * k, v, out and the strides multiples of 16 bytes, the strides positive. */
 VLA_API int32_t vla_cuda_prompt_attention(void* out, const void* q, int64_t q_tok, int64_t q_head,
                                           const void* k, int64_t k_tok, int64_t k_head,
                                           const void* v, int64_t v_tok, int64_t v_head, int32_t type,
@@ -299,7 +302,12 @@ VLA_API int32_t vla_cuda_kv4_read(const void* cache, int64_t n_pages, int32_t pa
  * sequence b sees its first lens[b] tokens, or with causal != 0 the first
  * clamp(lens[b] - queries + 1 + i, 0, lens[b]) (the new tokens are the last ones
  * of the cache). out [batch][queries][n_q][head_dim], same type as q (any); a
- * query that sees nothing gives zeros. A page index outside the cache is not read: its tokens
+ * query that sees nothing gives zeros, one that sees a score of NaN or +infinity
+ * gives NaN. For the matrix products q and weight * scale are held in 22 bits (F32;
+ * F16: weight * scale alone, q as it is), or the weight and its product with the
+ * scale in 11 bits each (BF16). The keys are shared out over the GPU by
+ * max_pages, not by lens: a table much wider than the longest sequence leaves
+ * part of it idle. A page index outside the cache is not read: its tokens
  * are left out and the device status word is set. Bytes of the cache past
  * lens[b] may hold anything. `ws`: workspace_bytes device bytes, 16-byte
  * aligned (NULL where that is 0); calls that may overlap on the GPU need

@@ -626,12 +626,14 @@ cudaError_t kv4_launch(const Kv4AttDev& p, dim3 grid, cudaStream_t st) {
     return launch_k(kv4_attention_kernel<NG, T>, grid, dim3(kKaThreads), ka_smem<NG>(), st, p);
 }
 
-// Keys a CTA takes. Three CTAs are resident on an SM: chunks down to a tile of
-// each warp fill one wave of them (latency: one sequence of 1021 tokens, 5 heads:
-// 6.9 us in 8 chunks); beyond that they only even out the tail, which pays down to
-// chunks of about 900 keys (16 sequences of up to 8192, 8 heads: 26 us in 10
-// chunks of 896, 30 in 5, 29 in 19) and not at 128 (8 sequences of 256 with 19
-// row tiles: 12 us whole, 17 in two).
+// Keys a CTA takes, from the width of the table (the lengths are on the device).
+// Chunks down to a tile of each warp fill one wave of three CTAs an SM (fp32
+// queries have two: theirs is a wave and a half). Latency: one sequence of 1021
+// tokens, 5 heads: 6.9 us in 8 chunks, 7.2 in 4, 10.3 whole. Beyond a wave chunks
+// only even out the tail, which pays while they stay near 1000 keys (16
+// sequences of up to 8192, 8 heads: 24.3 us in 8 chunks of 1024; 896: 25.5,
+// 1664: 29.6, 512: 28.5, whole: 66) and not at 128 (8 sequences of 256 with 19 row
+// tiles: 12.3 us whole, 21.2 in chunks of 128).
 int kv4_chunk(int batch, int row_ctas, long long max_len) {
     const long long tile = (long long)kKaTile * kKaWarps, ctas = (long long)batch * row_ctas;
     const long long fill = std::min((148 * 3 + ctas - 1) / ctas, max_len / tile);

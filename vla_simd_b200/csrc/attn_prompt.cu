@@ -6,9 +6,10 @@
 // both products on tcgen05 (128 x 64 x D and 128 x D x 64, accumulators in TMEM),
 // P written back over S's columns as the A operand of the second one, so scores
 // and weights never leave the SM. 16384 tokens, 32 heads over 8 of 128, causal:
-// 1.82 ms, 1.2 PFLOP/s (72 % of a large library product's rate) where the power
-// cap allows; a step of 64 keys takes the two tiles 1750 cycles, the tensor core
-// 1400 of them, the rest is the softmax's instruction latency.
+// 1.76 to 2.04 ms by the card and its power cap, 1.08 to 1.25 PFLOP/s (64 to 75 %
+// of a large library product's burst rate); a step of 64 keys takes the two tiles
+// 1750 cycles, the tensor core 1400 of them, the rest is the softmax's
+// instruction latency.
 //
 // A CTA has two 128-row tiles of one key head. A tile's rows are (query, head of
 // the group) pairs, token-major: the keys of a group are loaded once for all of
@@ -208,8 +209,9 @@ __device__ __forceinline__ float2 ex2_poly(float2 x) {
     return p;
 }
 
-// of 8 pairs of weights, how many the FMA pipe makes (0: 1870 us, 2: 1842, 3: 1815, 4: 1836 at 16384 tokens, 32
-// heads over 8 of 128: the SFUs alone are as long as the tensor core, the polynomial costs issue slots)
+// of 8 pairs of weights, how many the FMA pipe makes: the SFUs alone are as long as the tensor core, the polynomial
+// costs issue slots. Four runs each in turn, 32 heads over 8 of 128, 16384 tokens (median, range) and a ragged batch of
+// 8: 0: 1885 us (1848..1973), 105; 2: 1821 (1801..1947), 102; 3: 1785 (1757..1830), 100.5; 4: 1811 (1810..1845), 102
 constexpr int kPaPoly = 3;
 
 // What a CTA works on: tile t has rows of queries [tok[t], tok[t] + n_tok[t])

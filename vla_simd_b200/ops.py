@@ -338,7 +338,8 @@ def _tma_heads(x):
 
 def prompt_attention(q, k, v, cu_q, cu_k=None, scale=None, causal=True, prefix=None):
     """Attention over packed prompts: q [Tq, n_q, d], k / v [Tk, n_kv, d] (fp16 or bf16), cu_q / cu_k int32
-    [n_seq + 1] (cu_k defaults to cu_q), prefix int32 [n_seq] or None. Returns [Tq, n_q, d]."""
+    [n_seq + 1] (cu_k defaults to cu_q), prefix int32 [n_seq] or None. Returns [Tq, n_q, d]; its rows outside every
+    sequence (before cu_q[0], from cu_q[-1] on) are not written and hold anything."""
     (q, qs), (k, ks), (v, vs) = _tma_heads(q), _tma_heads(k), _tma_heads(v)
     Tq, n_q, d = q.shape
     Tk, n_kv, dk = k.shape
@@ -411,7 +412,8 @@ def kv4_read(cache, slots, dtype=torch.float32):
 
 def kv4_attention(q, cache, table, lens, scale=None, causal=True):
     """Attention of new tokens over the 4-bit cache: q [B, n_q, d] or [B, queries, n_q, d], table int32 [B, pages],
-    lens int32 [B] (tokens in the cache, the new ones among them). Returns q's shape and type."""
+    lens int32 [B] (tokens in the cache, the new ones among them). Returns q's shape and type. The work is planned by
+    the table's width: hand over the columns in use (table[:, :n], no copy) of one made for much longer sequences."""
     n_pages, n_kv, page, d = _cache(cache)
     shape = q.shape
     _need(len(shape) in (3, 4) and shape[-1] == d, "q has to be [batch, (queries,) n_q, head_dim] of the cache's width")
