@@ -104,8 +104,9 @@ class PromptedDecoder:
         self.lens += 1
         pos = self.next_pos.expand(3, -1).int().contiguous()
         self.next_pos = self.next_pos + 1
+        table = self.table[:, :-(-self.longest // self.page)]   # the pages in use: the kernel plans by its width
         h = self._layers(self.embed[tokens], pos, slots,
-                         lambda q, k, v, cache: ops.kv4_attention(q, cache, self.table, self.lens))
+                         lambda q, k, v, cache: ops.kv4_attention(q, cache, table, self.lens))
         return ops.dense_linear_i8(h, *self.head)
 
 
