@@ -31,6 +31,7 @@
 // saw no key.
 #include "serve_ops.h"
 #include "launch.cuh"
+#include "serve_math.cuh"
 #include "sm100.cuh"
 
 #include <algorithm>
@@ -45,12 +46,6 @@ namespace {
 constexpr int kKaWarps = 4, kKaThreads = 32 * kKaWarps;
 constexpr int kKaTile = 32, kKaBlocks = kKaTile / kKv4Block;   // tokens a warp takes at a time
 constexpr int kKaStages = 3;
-
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                         uint32_t b1) {

@@ -35,6 +35,7 @@
 #include "serve_ops.h"
 #include "gemm_i8.h"
 #include "launch.cuh"
+#include "serve_math.cuh"
 #include "sm100.cuh"
 
 #include <atomic>
@@ -165,14 +166,6 @@ template <int N>
 __device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(N)); }
 template <int N>
 __device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(N)); }
-
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-    float2 d;
-    asm("add.rn.f32x2 %0, %1, %2;"
-        : "=l"(reinterpret_cast<unsigned long long&>(d))
-        : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
-    return d;
-}
 
 // The registers of a tcgen05.ld are there once tmem_ld_wait() has returned: no
 // use of them may be moved in front of it.

@@ -3,10 +3,8 @@
 // is HBM at prompt sizes and the launch at single tokens.
 #include "serve_ops.h"
 #include "launch.cuh"
+#include "serve_math.cuh"
 #include "sm100.cuh"
-
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
 
 #include <algorithm>
 #include <climits>
@@ -16,33 +14,11 @@ namespace vsb {
 
 namespace {
 
-__device__ __forceinline__ float to_f(float x) { return x; }
-__device__ __forceinline__ float to_f(__half x) { return __half2float(x); }
-__device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
-template <typename T>
-__device__ __forceinline__ T from_f(float x);
-template <>
-__device__ __forceinline__ float from_f<float>(float x) { return x; }
-template <>
-__device__ __forceinline__ __half from_f<__half>(float x) { return __float2half_rn(x); }
-template <>
-__device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
-
 // N consecutive elements as one access (p aligned to N * sizeof(T), at most 16 bytes each)
 template <typename T, int N>
 struct alignas(N * sizeof(T) > 16 ? 16 : N * sizeof(T)) Pack {
     T v[N];
 };
-
-template <typename F>
-cudaError_t by_type(int type, F&& f) {
-    switch (type) {
-        case kF32: return f(float{});
-        case kF16: return f(__half{});
-        case kBF16: return f(__nv_bfloat16{});
-    }
-    return cudaErrorInvalidValue;
-}
 
 // ------------------------------------------------- norm + rotary positions
 // y = x * rsqrt(mean(x^2) + eps) * w over the d channels of one head, then pair
@@ -79,26 +55,6 @@ __device__ __forceinline__ void load_quad(const float* p, float2 (&x)[2]) {
     x[1] = make_float2(v.z, v.w);
 }
 template <typename T>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi);
-template <>
-__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
-    uint32_t r;
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
-}
-template <>
-__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
-    uint32_t r;
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
-}
-__device__ __forceinline__ float2 unpack2(uint32_t w, __nv_bfloat16) {
-    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
-}
-__device__ __forceinline__ float2 unpack2(uint32_t w, __half) {
-    return __half22float2(*reinterpret_cast<const __half2*>(&w));
-}
-template <typename T>
 struct Quad {   // 16-bit
     uint2 w;
     __device__ __forceinline__ float2 lo() const { return unpack2(w.x, T{}); }
@@ -120,22 +76,6 @@ struct Quad<float> {
         return q;
     }
 };
-
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-    float2 d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;"
-        : "=l"(reinterpret_cast<unsigned long long&>(d))
-        : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)),
-          "l"(reinterpret_cast<unsigned long long&>(c)));
-    return d;
-}
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-    float2 d;
-    asm("mul.rn.f32x2 %0, %1, %2;"
-        : "=l"(reinterpret_cast<unsigned long long&>(d))
-        : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
-    return d;
-}
 
 // A warp has one token (or a share of its heads). GS lanes (the power of two >= d
 // / 8) have a row; lane l the two quads of channels [c0, c0 + 4) and [c1, c1 + 4)
@@ -405,17 +345,6 @@ __device__ __forceinline__ __half* kv4_key_min(const Kv4At& at, int ng, int g) {
 // scales of the keys at byte 256 ng, of the values at 576 ng, minima of the values at 608 ng
 __device__ __forceinline__ __half* kv4_by_quad(const Kv4At& at, int byte) {
     return reinterpret_cast<__half*>(at.block + byte) + at.by_quad;
-}
-
-__device__ __forceinline__ float min_nan(float a, float b, float c) {   // NaN if one is
-    float r;
-    asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-    return r;
-}
-__device__ __forceinline__ float max_nan(float a, float b, float c) {
-    float r;
-    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-    return r;
 }
 
 // codes of 8 channels (one nibble each) and the group's s, m; the group is
