@@ -105,3 +105,11 @@ def test_prompt_refuses_totals_past_32_bits():
     for n in (2 ** 30 + 1, 2 ** 31 - 1):
         assert prompt(lib(), tq=n, n_seq=0) == VLA_ERR_ARG and prompt(lib(), tk=n, n_seq=0) == VLA_ERR_ARG
     assert prompt(lib(), tq=2 ** 30, tk=2 ** 30, n_seq=0) == 0   # no sequence: nothing is launched
+
+
+@pytest.mark.parametrize("batch,queries,n_q,n_kv,d,pages,page,chunks", [
+    (1, 1, 15, 5, 64, 64, 16, 8), (8, 50, 15, 5, 64, 5, 64, 1), (16, 1, 32, 8, 128, 128, 64, 8), (48, 1, 32, 8, 128, 128, 128, 4),
+])
+def test_chunks_that_the_stated_times_speak_of(batch, queries, n_q, n_kv, d, pages, page, chunks):
+    size = lib().vla_cuda_kv4_attention_workspace_bytes(batch, queries, n_q, n_kv, d, pages, page)
+    assert size == (0 if chunks == 1 else batch * queries * n_q * chunks * (d + 2) * 4)
