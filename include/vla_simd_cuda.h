@@ -251,9 +251,12 @@ VLA_API int32_t vla_cuda_qk_norm_rope(void* q_out, void* k_out, int32_t out_type
  * whatever they hold. A score that is NaN or +infinity makes its row NaN, as do
  * scores that are all -infinity. Rows outside every sequence are not written.
  * type F16 or BF16: the weights are rounded to it for the product with v, and 3
- * of 8 come from a polynomial good to 2^-18.5 (F16) or 2^-13.7 (BF16). head_dim
- * a multiple of 8, at most 128; total_q and total_k at most 2^30; addresses of q,
- * k, v, out and the strides multiples of 16 bytes, the strides positive. */
+ * of 8 come from a polynomial good to 2^-18.5 (F16) or 2^-13.7 (BF16); F16 ones
+ * below 2^-20 of a row's largest are good to 2^-31 of it. The tensor core
+ * truncates its 32-bit sums: past 65536 keys that is more than F16's rounding
+ * (2e-3 of sum weight |v| at 131072 keys). head_dim a multiple of 8, at most 128;
+ * total_q and total_k at most 2^30; addresses of q, k, v, out and the strides
+ * multiples of 16 bytes, the strides positive. */
 VLA_API int32_t vla_cuda_prompt_attention(void* out, const void* q, int64_t q_tok, int64_t q_head,
                                           const void* k, int64_t k_tok, int64_t k_head,
                                           const void* v, int64_t v_tok, int64_t v_head, int32_t type,

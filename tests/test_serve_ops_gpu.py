@@ -623,3 +623,21 @@ def test_kv4_attention_queries_of_any_size(dtype, power):
     cache, table, kv = make_cache(g, [300], 2, 64, 64)
     q = randn(g, 1, 1, 4, 64, dtype=dtype).clamp(-7.9, 7.9).double() * 2.0 ** power
     check_decode(q.to(dtype), cache, table, kv, True, scale=2.0 ** (-power - 3))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("T", [1000, 4096, 16384])
+@pytest.mark.parametrize("rest", [1 / 8, 1 / 90, 1 / 400])
+def test_prompt_many_small_weights_beside_a_large_one(dtype, T, rest):
+    """A first key of nearly all the weight, and the others, which share `rest` of it: down to 2^-22 each, in channels
+    that the first key's value may leave to them alone."""
+    g = gen(19)
+    d = 64
+    q, k = torch.zeros(3, 1, d, device="cuda", dtype=dtype), torch.zeros(T, 1, d, device="cuda", dtype=dtype)
+    q[:, 0, 0], q[:, 0, 1] = 1.0, 0.03125
+    score = -math.log(rest / T)
+    k[0, 0, 0] = math.floor(score)                                  # the score in two parts that bf16 holds
+    k[0, 0, 1] = 32 * (score - math.floor(score))
+    v = (1.0 + randn(g, T, 1, d)).to(dtype)
+    check_prompt(q, k, v, [3], [T], causal=False, scale=1.0)
+    check_prompt(q, k, torch.ones_like(v), [3], [T], causal=False, scale=1.0)

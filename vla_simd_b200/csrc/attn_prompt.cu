@@ -26,7 +26,7 @@
 // cycles, and its products, 1400, followed one another.)
 //
 // m only follows the true maximum when it is more than 2^8 behind (P then stays
-// below 2^8, far inside bf16 and fp16): O is rescaled in TMEM that rarely, by
+// below 2^8, or 2^14 with fp16's factor, inside bf16 and fp16): O is rescaled in TMEM that rarely, by
 // the softmax threads themselves.
 //
 // A score that is NaN or +infinity makes its row NaN, and so do scores that are
@@ -449,6 +449,9 @@ prompt_tc_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__ C
         const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t tS = tmem + 128 * t + lane_base, tO = tmem + 256 + 128 * t + lane_base;
         const float c = a.scale_log2, slack = 8.0f / c;
+        // fp16 weights carry 2^6 (at most 2^14, with m 2^8 behind): beside a key of weight 1 the others are good to 2^-31
+        // of it. Without, to 2^-25: 16384 keys that share a 90th were off by 2 % of themselves, now by 2^-10.
+        constexpr float kUp = kBf16 ? 0.f : 6.f;
         float m = -INFINITY, l = 0.f;
         bool ok = true;
         // the ring is freed in pairs: K tile 0, then p: V tile p - 1 and K tile p. When the scores of step 2 p +
@@ -490,7 +493,7 @@ prompt_tc_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__ C
             const float top = max_nan(mx[0], mx[1], mx[1]);
             // a seen score that is NaN or +infinity: from here on the row's sum, and with it the row, is NaN
             if (!(top <= 3.402823466e38f)) l = __int_as_float(0x7fffffff);
-            if (__any_sync(0xffffffffu, top > m + slack || (m == -INFINITY && top > m))) {
+            if (__any_sync(0xffffffffu, top - m > slack)) {   // m = -infinity: any finite top
                 const float mn = fmaxf(m, top);
                 if (i > 0) {
                     // rescale O once the products so far are in (this step's are not issued before its P is there)
@@ -514,7 +517,7 @@ prompt_tc_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__ C
                 }
                 m = mn;
             }
-            const float mc = m == -INFINITY ? 0.f : -m * c;
+            const float mc = m == -INFINITY ? 0.f : kUp - m * c;
             const float2 c2 = make_float2(c, c), mc2 = make_float2(mc, mc);
             float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
             uint32_t p[32];
